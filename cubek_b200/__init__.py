@@ -3,7 +3,7 @@
 
 Modules mirror the reference crate: ``scheme``, ``quantize``, ``dequantize``, ``layout``.
 """
-from . import dequantize, quantize, scheme  # noqa: F401
+from . import dequantize, grouped_linear, linear, quantize, scheme  # noqa: F401
 from ._ffi import LaunchError, QuantPanic  # noqa: F401
 from .scheme import (BlockSize, ElemType, Flex32, QuantLevel, QuantMode, QuantParam, QuantScheme,  # noqa: F401
                      QuantStore, QuantValue)

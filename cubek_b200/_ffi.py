@@ -70,6 +70,7 @@ class QuantPanic(AssertionError):
 
 _lib = None
 
+_T = C.POINTER(QkTensor)
 _SIGNATURES = {
     "qk_num_quants": (C.c_int, [C.POINTER(QkScheme)]),
     "qk_value_range": (C.c_int, [C.c_int, C.POINTER(C.c_float), C.POINTER(C.c_float)]),
@@ -103,6 +104,13 @@ _SIGNATURES = {
                                                       C.c_size_t, C.c_int]),
     "qk_host_roundtrip_staging_bytes_batch": (C.c_size_t, [C.c_int, C.POINTER(QkTensor), C.POINTER(QkScheme), C.c_int]),
     "qk_into_contiguous_packed": (C.c_int, [C.POINTER(QkTensor)] * 2 + [C.POINTER(C.c_int64), C.c_int, C.c_int, C.c_void_p]),
+    "qk_linear": (C.c_int, [_T] * 3 + [C.POINTER(QkScheme)] + [_T] * 2 + [C.c_int] + [_T] * 2 + [C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "qk_grouped_linear": (C.c_int, [_T] * 4 + [C.POINTER(QkScheme)] + [_T] * 2 + [C.c_int] + [_T] * 2 + [C.c_int, C.c_void_p, C.c_size_t,
+                                                                                                       C.c_void_p]),
+    "qk_linear_backward": (C.c_int, [_T] * 3 + [C.POINTER(QkScheme), C.c_int] + [_T] * 4 + [C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "qk_grouped_linear_backward": (C.c_int, [_T] * 4 + [C.POINTER(QkScheme), C.c_int] + [_T] * 4 + [C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "qk_linear_workspace_bytes": (C.c_size_t, [_T] * 2 + [C.POINTER(QkScheme), C.c_int]),
+    "qk_linear_backward_workspace_bytes": (C.c_size_t, [_T] * 2 + [C.POINTER(QkScheme)] + [C.c_int] * 4),
     "qk_strerror": (C.c_char_p, [C.c_int]),
     "qk_version": (C.c_char_p, []),
     "qk_launch_count": (C.c_uint64, []),
@@ -181,6 +189,14 @@ class CTensor:
 
     def ref(self):
         return C.byref(self.c)
+
+
+def optional(t: TensorHandleRef | None):
+    """(keeper, pointer argument) of a tensor that may be absent."""
+    if t is None:
+        return None, None
+    c = CTensor(t)
+    return c, c.ref()
 
 
 def c_tensors(*tensors: TensorHandleRef) -> Sequence[CTensor]:

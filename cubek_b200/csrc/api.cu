@@ -14,6 +14,7 @@
 
 #include "../../include/cubek_quant_b200_testing.h"
 #include "dequantize_kernels.cuh"
+#include "host_checks.cuh"
 #include "misc_kernels.cuh"
 #include "quantize_kernels.cuh"
 
@@ -115,7 +116,7 @@ static int sm_count_of_current_device()
     return n;
 }
 
-static LaunchCfg current_cfg()
+LaunchCfg current_cfg()
 {
     LaunchCfg c;
     c.threads = g_tune[TUNE_THREADS].load();
@@ -131,11 +132,11 @@ static LaunchCfg current_cfg()
     return c;
 }
 
-static inline int cuda_status(cudaError_t e) { return e == cudaSuccess ? QK_OK : QK_ERR_CUDA + (int)e; }
-static inline void count_launch(int n = 1) { g_launches.fetch_add((uint64_t)n, std::memory_order_relaxed); }
+int cuda_status(cudaError_t e) { return e == cudaSuccess ? QK_OK : QK_ERR_CUDA + (int)e; }
+void count_launch(int n) { g_launches.fetch_add((uint64_t)n, std::memory_order_relaxed); }
 
 // ---- scheme helpers ----------------------------------------------------------------------------
-static int dtype_size(int dt) { return dt == QK_F32 ? 4 : (dt == QK_F16 || dt == QK_BF16) ? 2 : 0; }
+int dtype_size(int dt) { return dt == QK_F32 ? 4 : (dt == QK_F16 || dt == QK_BF16) ? 2 : 0; }
 
 static int value_bits(int value)
 {
@@ -147,7 +148,7 @@ static int value_bits(int value)
     }
 }
 
-static int num_quants(const QkScheme *s)
+int num_quants(const QkScheme *s)
 {
     const int bits = value_bits(s->value);
     if (bits == 0) return 0;
@@ -156,7 +157,7 @@ static int num_quants(const QkScheme *s)
     return 0;
 }
 
-static int kind_of(const QkScheme *s)
+int kind_of(const QkScheme *s)
 {
     if (s->store == QK_STORE_U32) {
         const int bits = value_bits(s->value);
@@ -172,7 +173,7 @@ static int kind_of(const QkScheme *s)
 }
 
 // The checks `launch_ref` performs by pattern matching (quantize.rs:185-220).
-static int check_scheme(const QkScheme *s)
+int check_scheme(const QkScheme *s)
 {
     if (value_bits(s->value) == 0) return QK_ERR_UNSUPPORTED_SCHEME;
     if (s->store != QK_STORE_U32 && s->store != QK_STORE_NATIVE) return QK_ERR_UNSUPPORTED_SCHEME;
@@ -195,7 +196,7 @@ static long long numel(const QkTensor *t)
     return n;
 }
 
-static bool is_contiguous(const QkTensor *t)
+bool is_contiguous(const QkTensor *t)
 {
     long long expect = 1;
     for (int d = t->rank - 1; d >= 0; --d) {
@@ -233,7 +234,7 @@ static bool is_dense_permutation(const QkTensor *t)
 
 // Rows (runs along the last dim) contiguous, rows a constant number of elements apart: a column slice
 // of a wider matrix, a matrix with padded rows.  Leading dims must step uniformly over the rows.
-static bool is_row_strided(const QkTensor *t, long long *row_stride)
+bool is_row_strided(const QkTensor *t, long long *row_stride)
 {
     const int r = t->rank;
     if (r < 2 || (t->shape[r - 1] != 1 && t->strides[r - 1] != 1)) return false;
@@ -276,7 +277,7 @@ static long long fill_transposed_tiles(Transposed &tr, const QkTensor *t, long l
     return row_tiles * unit_tiles;
 }
 
-static int check_tensor(const QkTensor *t, int elem_size)
+int check_tensor(const QkTensor *t, int elem_size)
 {
     if (!t || !t->shape || !t->strides) return QK_ERR_NULL;
     if (t->rank < 1 || t->rank > QK_MAX_RANK) return QK_ERR_SHAPE;

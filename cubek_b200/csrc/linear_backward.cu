@@ -1,0 +1,131 @@
+// dz = dy * act'(z) and the bias gradient: what the backward pass does before its product, dx = dz W.
+//
+// One pass over dy and z, memory bound: 2 (dy) + 2 (z) + 2 (dz) bytes per element, sums of the columns on the way.
+// A CTA takes one strip of columns and one slice of an expert's rows; a column's sum is accumulated in f32 from the
+// unrounded products, first per thread, then over the CTA, and where an expert has several slices their partial sums
+// are added in slice order by a second small kernel: the same bits every time.
+#include "linear_backward.cuh"
+
+namespace qk {
+
+// VEC: elements per access.  8 row lanes of 32 threads; a strip is 32 * VEC columns.
+template <int FDT, int VEC> __global__ void __launch_bounds__(256) activation_backward_kernel(const ActBackwardArgs a)
+{
+    using F = typename ElemOf<FDT>::type;
+    __shared__ float part[8][32 * VEC];
+    pdl_entry();
+    const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+    const int col = (blockIdx.x * 32 + tx) * VEC, e = blockIdx.y, slice = blockIdx.z;
+    LinearArgs rows = {};
+    rows.offsets = a.offsets;
+    rows.offsets64 = a.offsets64;
+    rows.rows = a.rows;
+    int lo, hi;
+    expert_rows(rows, e, lo, hi);
+    const int per = (hi - lo + a.slices - 1) / a.slices;
+    const long long first = lo + (long long)slice * per;
+    const int last = (int)min((long long)hi, first + per);
+    float sum[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
+    if (col < a.n) {
+        for (int r = (int)min(first, (long long)hi) + ty; r < last; r += 8) {
+            float g[VEC], z[VEC];
+            if constexpr (VEC == 8) {
+                const Vec16 v = ldg128_stream(static_cast<const F *>(a.grad) + r * a.grad_stride + col);
+                widen16<FDT>(v, g);
+                if (a.act != QK_ACT_IDENTITY) {
+                    const Vec16 u = ldg128_stream(static_cast<const F *>(a.pre) + r * a.pre_stride + col);
+                    widen16<FDT>(u, z);
+                }
+            } else {
+                g[0] = (float)static_cast<const F *>(a.grad)[r * a.grad_stride + col];
+                if (a.act != QK_ACT_IDENTITY) z[0] = (float)static_cast<const F *>(a.pre)[r * a.pre_stride + col];
+            }
+            if (a.act != QK_ACT_IDENTITY) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) g[i] *= activation_slope(a.act, z[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) sum[i] += g[i];
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                F *to = static_cast<F *>(d ? a.dz2 : a.dz);
+                if (to == nullptr) continue;
+                to += r * (d ? a.dz2_stride : a.dz_stride) + col;
+                if constexpr (VEC == 8) {
+                    uint4 v;
+                    v.x = h2_pack<FDT>(g[0], g[1]);
+                    v.y = h2_pack<FDT>(g[2], g[3]);
+                    v.z = h2_pack<FDT>(g[4], g[5]);
+                    v.w = h2_pack<FDT>(g[6], g[7]);
+                    *reinterpret_cast<uint4 *>(to) = v;
+                } else {
+                    *to = (F)g[0];
+                }
+            }
+        }
+    }
+    if (a.grad_bias == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) part[ty][tx * VEC + i] = sum[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
+        const int c = blockIdx.x * 32 * VEC + i;
+        if (c >= a.n) continue;
+        float s = part[0][i];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) s += part[j][i];
+        if (a.slices > 1) a.partial[((long long)e * a.slices + slice) * a.n + c] = s;
+        else static_cast<F *>(a.grad_bias)[e * a.grad_bias_expert + c * a.grad_bias_stride] = (F)s;
+    }
+}
+
+template <int FDT> __global__ void __launch_bounds__(256) bias_gradient_kernel(const ActBackwardArgs a)
+{
+    using F = typename ElemOf<FDT>::type;
+    pdl_entry();
+    const int c = blockIdx.x * 256 + threadIdx.x, e = blockIdx.y;
+    if (c >= a.n) return;
+    float s = 0.0f;
+    for (int i = 0; i < a.slices; ++i) s += a.partial[((long long)e * a.slices + i) * a.n + c];
+    static_cast<F *>(a.grad_bias)[e * a.grad_bias_expert + c * a.grad_bias_stride] = (F)s;
+}
+
+// A few hundred CTAs in all, and no slice below 64 rows of an evenly filled expert.
+int bias_slices(long long rows, long long n, int experts)
+{
+    const long long strips = (n + 255) / 256;
+    long long s = 592 / (strips * experts);
+    const long long most = rows / (64ll * experts);
+    if (s > most) s = most;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+template <int FDT> static cudaError_t launch_dtype(const ActBackwardArgs &a, const LaunchCfg &cfg, cudaStream_t stream, int *launches)
+{
+    const bool vec = a.vec != 0;
+    const int strip = vec ? 256 : 32;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((unsigned)((a.n + strip - 1) / strip), (unsigned)a.experts, (unsigned)a.slices);
+    c.blockDim = dim3(256);
+    c.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = attr;
+    c.numAttrs = cfg.pdl ? 1 : 0;
+    cudaError_t err = vec ? cudaLaunchKernelEx(&c, activation_backward_kernel<FDT, 8>, a) : cudaLaunchKernelEx(&c, activation_backward_kernel<FDT, 1>, a);
+    *launches = 1;
+    if (err != cudaSuccess || a.grad_bias == nullptr || a.slices == 1) return err;
+    c.gridDim = dim3((unsigned)((a.n + 255) / 256), (unsigned)a.experts, 1);
+    *launches = 2;
+    return cudaLaunchKernelEx(&c, bias_gradient_kernel<FDT>, a);
+}
+
+cudaError_t launch_activation_backward(int fdt, const ActBackwardArgs &a, const LaunchCfg &cfg, cudaStream_t stream, int *launches)
+{
+    return fdt == QK_F16 ? launch_dtype<QK_F16>(a, cfg, stream, launches) : launch_dtype<QK_BF16>(a, cfg, stream, launches);
+}
+
+}  // namespace qk

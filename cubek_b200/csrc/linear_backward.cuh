@@ -1,0 +1,28 @@
+// Arguments of the activation-gradient and bias-gradient kernels (linear_backward.cu).
+#pragma once
+
+#include "linear_kernels.cuh"
+
+namespace qk {
+
+struct ActBackwardArgs {
+    const void *grad;   // [rows, n]
+    long long grad_stride;
+    const void *pre;    // [rows, n]; unread with QK_ACT_IDENTITY
+    long long pre_stride;
+    void *dz, *dz2;     // up to two places for the products, rounded to F; nullptr: not written
+    long long dz_stride, dz2_stride;
+    void *grad_bias;    // [experts, n]; nullptr: no sums
+    long long grad_bias_stride, grad_bias_expert;
+    float *partial;     // [experts, slices, n] where slices > 1
+    int slices;
+    int n, rows, act, experts, vec;
+    const void *offsets;
+    int offsets64;
+};
+
+int bias_slices(long long rows, long long n, int experts);
+cudaError_t launch_activation_backward(int fdt, const ActBackwardArgs &a, const LaunchCfg &cfg, cudaStream_t stream, int *launches);
+cudaError_t launch_linear_product(int fdt, int kind, bool backward, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream);
+
+}  // namespace qk

@@ -285,6 +285,68 @@ size_t qk_host_roundtrip_staging_bytes_batch(int count, const QkTensor *inputs, 
 int qk_into_contiguous_packed(const QkTensor *input, const QkTensor *output, const int64_t *shape, int rank, int packing,
                               void *stream);
 
+/*
+ * Products with quantized weights: y = act(x W^T + bias) + residual, and their gradients.  The reference hands the
+ * same operand - `MatmulInputHandleRef::quantized(data, scale, shape, scheme, ..)`
+ * (crates/cubek-matmul/src/base.rs:436-452) - to its matmul; bias, activation, residual and experts have no
+ * counterpart there.
+ *
+ * W [N, K] is held as qk_quantize writes it and is, to the bit, the tensor that qk_dequantize returns in the type of x:
+ * code times scale, the scale rounded to the type of x, the product rounded to it.  Products are summed in f32; y is
+ * rounded once, after bias, activation and residual.  The same call on the same inputs gives the same bits.
+ *   input     x [.., K], `dtype` f16 or bf16; rows contiguous and a constant stride apart (so are those of every
+ *             other float matrix here); leading dims are rows
+ *   values    [N, K / num_quants]; rows contiguous, any row stride
+ *   params    [1] per tensor, else one scale per block, any non-negative strides; blocks are 1-D (along K) or tiles
+ *             [block_rows, block_cols]; their extent along K is a multiple of 8 or covers K (else QK_ERR_BLOCK_SIZE)
+ *   bias      [N], typed as x; NULL: none
+ *   residual  [.., N], typed as x; NULL: none; may be the output itself
+ *   output    y [.., N], typed as x; overlaps no input but `residual`
+ *   pre       [.., N], receives x W^T + bias (rounded), which the gradient of the activation needs; NULL: not kept
+ * A column-major operand (packed along N) is QK_ERR_LAYOUT: qk_into_contiguous_packed makes it row-major.
+ */
+typedef enum {
+    QK_ACT_IDENTITY = 0, QK_ACT_RELU = 1, QK_ACT_GELU = 2 /* z Phi(z) */, QK_ACT_GELU_TANH = 3 /* its tanh form */, QK_ACT_SILU = 4
+} QkActivation;
+int qk_linear(const QkTensor *input, const QkTensor *values, const QkTensor *params, const QkScheme *scheme, const QkTensor *bias,
+              const QkTensor *residual, int activation, const QkTensor *output, const QkTensor *pre, int dtype, void *workspace,
+              size_t workspace_bytes, void *stream);
+
+/*
+ * The same for E <= QK_LINEAR_MAX_EXPERTS experts: values [E, N, K / num_quants], params with a leading dim per block
+ * (one scale in all per tensor), bias [E, N].  The rows of x are sorted by expert: rows offsets[e] .. offsets[e + 1]
+ * use W[e] and bias[e].  `offsets` is a device array of E + 1 int32 or int64 in ascending order, 0 <= offsets <= rows
+ * (others are clamped); an expert may have no rows.  Rows outside [offsets[0], offsets[E]) are left as they were in
+ * every output.
+ */
+#define QK_LINEAR_MAX_EXPERTS 1024
+int qk_grouped_linear(const QkTensor *input, const QkTensor *offsets, const QkTensor *values, const QkTensor *params, const QkScheme *scheme,
+                      const QkTensor *bias, const QkTensor *residual, int activation, const QkTensor *output, const QkTensor *pre, int dtype,
+                      void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Gradients.  With g = dL/dy:  dz = g act'(pre),  grad_input = dz W,  grad_bias = sum of dz over the rows (of the expert),
+ * and the gradient of the residual is g itself.  Codes are integers and scales constants: they have no gradient here;
+ * `grad_pre` receives dz (rounded) for callers that train weights behind the codes.
+ * dz is rounded to the type of x before the product (it is an operand of the tensor cores); grad_bias sums the
+ * unrounded ones in f32 and is rounded once.
+ *   pre        what the forward pass left in `pre`; may be NULL with QK_ACT_IDENTITY
+ *   grad_input, grad_bias, grad_pre   each may be NULL: not computed.  grad_bias of an expert without rows is zero.
+ */
+int qk_linear_backward(const QkTensor *grad_output, const QkTensor *values, const QkTensor *params, const QkScheme *scheme, int activation,
+                       const QkTensor *pre, const QkTensor *grad_input, const QkTensor *grad_bias, const QkTensor *grad_pre, int dtype,
+                       void *workspace, size_t workspace_bytes, void *stream);
+int qk_grouped_linear_backward(const QkTensor *grad_output, const QkTensor *offsets, const QkTensor *values, const QkTensor *params,
+                               const QkScheme *scheme, int activation, const QkTensor *pre, const QkTensor *grad_input,
+                               const QkTensor *grad_bias, const QkTensor *grad_pre, int dtype, void *workspace, size_t workspace_bytes,
+                               void *stream);
+
+/* Device workspace of these calls (16-byte aligned; `values` of rank 3 for the grouped forms).  It needs no
+ * initialisation and holds nothing between calls; calls that may overlap need one each. */
+size_t qk_linear_workspace_bytes(const QkTensor *input, const QkTensor *values, const QkScheme *scheme, int dtype);
+size_t qk_linear_backward_workspace_bytes(const QkTensor *grad_output, const QkTensor *values, const QkScheme *scheme, int activation,
+                                          int has_grad_bias, int has_grad_pre, int dtype);
+
 const char *qk_strerror(int status);
 const char *qk_version(void);
 
