@@ -110,7 +110,7 @@ _SIGNATURES = {
     "qk_linear_backward": (C.c_int, [_T] * 3 + [C.POINTER(QkScheme), C.c_int] + [_T] * 4 + [C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
     "qk_grouped_linear_backward": (C.c_int, [_T] * 4 + [C.POINTER(QkScheme), C.c_int] + [_T] * 4 + [C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
     "qk_linear_workspace_bytes": (C.c_size_t, [_T] * 2 + [C.POINTER(QkScheme), C.c_int]),
-    "qk_linear_backward_workspace_bytes": (C.c_size_t, [_T] * 2 + [C.POINTER(QkScheme)] + [C.c_int] * 4),
+    "qk_linear_backward_workspace_bytes": (C.c_size_t, [_T] * 2 + [C.POINTER(QkScheme), C.c_int, C.c_int, _T, C.c_int]),
     "qk_strerror": (C.c_char_p, [C.c_int]),
     "qk_version": (C.c_char_p, []),
     "qk_launch_count": (C.c_uint64, []),

@@ -130,7 +130,29 @@ static int check_offsets(const QkTensor *t, int experts, const void **ptr, int *
     return QK_OK;
 }
 
+static size_t round256(size_t v) { return (v + 255) & ~(size_t)255; }
+
 static bool even_words(const void *p, long long stride) { return reinterpret_cast<uintptr_t>(p) % 4 == 0 && stride % 2 == 0; }
+
+// Rows of x that do not start on 16 bytes are copied to ones that do (bulk tensor loads need it).
+static size_t copied_rows_bytes(long long rows, long long cols) { return round256((size_t)rows * ((cols + 7) / 8 * 8) * 2); }
+
+static int copy_rows(const Matrix &x, int dtype, void *to, long long stride, cudaStream_t stream)
+{
+    ActBackwardArgs b = {};
+    b.grad = x.ptr;
+    b.grad_stride = x.stride;
+    b.dz = to;
+    b.dz_stride = stride;
+    b.slices = bias_slices(x.rows, x.cols, 1);
+    b.n = (int)x.cols;
+    b.rows = (int)x.rows;
+    b.experts = 1;
+    int launches = 0;
+    const cudaError_t e = launch_activation_backward(dtype, b, current_cfg(), stream, &launches);
+    count_launch(launches);
+    return cuda_status(e);
+}
 
 static int run_product(int dtype, const QkScheme *s, bool backward, LinearArgs &a, cudaStream_t stream)
 {
@@ -161,6 +183,13 @@ static int linear_forward(const QkTensor *input, const QkTensor *offsets, bool g
     if (x.rows == 0 || a.n == 0) return QK_OK;
     a.x = x.ptr;
     a.x_stride = x.stride;
+    if (a.k > 0 && product_needs_aligned_rows(x.rows, x.ptr, x.stride)) {
+        if (!workspace || workspace_bytes < copied_rows_bytes(x.rows, x.cols)) return QK_ERR_WORKSPACE;
+        if (reinterpret_cast<uintptr_t>(workspace) % 16) return QK_ERR_ALIGN;
+        a.x = workspace;
+        a.x_stride = (x.cols + 7) / 8 * 8;
+        if ((rc = copy_rows(x, dtype, workspace, a.x_stride, stream)) != QK_OK) return rc;
+    }
     a.rows = (int)x.rows;
     a.contraction = a.k;
     a.feats = a.n;
@@ -183,12 +212,11 @@ struct BackwardPlan {
     int slices;
 };
 
-static size_t round256(size_t v) { return (v + 255) & ~(size_t)255; }
-
-static BackwardPlan plan_backward(long long rows, long long n, int experts, int activation, bool grad_bias, bool grad_pre)
+// `operand_aligned`: what the product would read otherwise, grad_pre or grad_output, can be loaded as it lies.
+static BackwardPlan plan_backward(long long rows, long long n, int experts, int activation, bool grad_bias, bool grad_pre, bool operand_aligned)
 {
     BackwardPlan p;
-    p.dz = activation != QK_ACT_IDENTITY && !grad_pre;
+    p.dz = (activation != QK_ACT_IDENTITY && !grad_pre) || !operand_aligned;
     p.dz_stride = (n + 7) / 8 * 8;
     size_t at = p.dz ? round256((size_t)rows * p.dz_stride * 2) : 0;
     p.partial_at = at;
@@ -218,7 +246,9 @@ static int linear_backward(const QkTensor *grad_output, const QkTensor *offsets,
     if (grad_bias && (rc = check_bias(grad_bias, dtype, grouped, a.experts, a.n, true, &b.grad_bias_stride, &b.grad_bias_expert)) != QK_OK)
         return rc;
     if (grouped && (rc = check_offsets(offsets, a.experts, &a.offsets, &a.offsets64)) != QK_OK) return rc;
-    const BackwardPlan plan = plan_backward(g.rows, a.n, a.experts, activation, grad_bias != nullptr, grad_pre != nullptr);
+    const Matrix &operand = activation != QK_ACT_IDENTITY && grad_pre ? dz : g;
+    const BackwardPlan plan = plan_backward(g.rows, a.n, a.experts, activation, grad_bias != nullptr, grad_pre != nullptr,
+                                            !product_needs_aligned_rows(operand.rows, operand.ptr, operand.stride));
     const bool product = grad_input && g.rows > 0 && a.k > 0;
     const bool needs = (plan.dz && product) || (grad_bias && plan.slices > 1);
     if (needs && (!workspace || workspace_bytes < plan.bytes)) return QK_ERR_WORKSPACE;
@@ -252,8 +282,8 @@ static int linear_backward(const QkTensor *grad_output, const QkTensor *offsets,
         if (e != cudaSuccess) return cuda_status(e);
     }
     if (!product) return QK_OK;
-    a.x = staged ? workspace : activation == QK_ACT_IDENTITY ? g.ptr : dz.ptr;
-    a.x_stride = staged ? plan.dz_stride : activation == QK_ACT_IDENTITY ? g.stride : dz.stride;
+    a.x = staged ? workspace : operand.ptr;
+    a.x_stride = staged ? plan.dz_stride : operand.stride;
     a.rows = (int)g.rows;
     a.contraction = a.n;
     a.feats = a.k;
@@ -300,19 +330,26 @@ int qk_grouped_linear_backward(const QkTensor *grad_output, const QkTensor *offs
                                workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
-size_t qk_linear_workspace_bytes(const QkTensor *input, const QkTensor *values, const QkScheme *scheme, int dtype) { return 0; }
+size_t qk_linear_workspace_bytes(const QkTensor *input, const QkTensor *values, const QkScheme *scheme, int dtype)
+{
+    if (!input || !values || !scheme) return 0;
+    qk::Matrix x;
+    if ((dtype != QK_F16 && dtype != QK_BF16) || qk::as_matrix(input, dtype, x) != QK_OK || x.rows == 0 || x.cols == 0) return 0;
+    return qk::product_needs_aligned_rows(x.rows, x.ptr, x.stride) ? qk::copied_rows_bytes(x.rows, x.cols) : 0;
+}
 
 size_t qk_linear_backward_workspace_bytes(const QkTensor *grad_output, const QkTensor *values, const QkScheme *scheme, int activation,
-                                          int has_grad_bias, int has_grad_pre, int dtype)
+                                          int has_grad_bias, const QkTensor *grad_pre, int dtype)
 {
-    if (!grad_output || !values || !grad_output->shape || !values->shape || grad_output->rank < 1 || grad_output->rank > QK_MAX_RANK ||
-        values->rank < 2 || values->rank > 3)
-        return 0;
-    long long rows = 1;
-    for (int d = 0; d < grad_output->rank - 1; ++d) rows *= grad_output->shape[d];
+    if (!grad_output || !values || !scheme || !values->shape || values->rank < 2 || values->rank > 3) return 0;
+    qk::Matrix g, z;
+    if ((dtype != QK_F16 && dtype != QK_BF16) || qk::as_matrix(grad_output, dtype, g) != QK_OK) return 0;
+    if (grad_pre && qk::as_matrix(grad_pre, dtype, z) != QK_OK) return 0;
     const long long experts = values->rank == 3 ? values->shape[0] : 1;
-    if (experts < 1 || experts > QK_LINEAR_MAX_EXPERTS || rows < 0) return 0;
-    return qk::plan_backward(rows, values->shape[values->rank - 2], (int)experts, activation, has_grad_bias != 0, has_grad_pre != 0).bytes;
+    if (experts < 1 || experts > QK_LINEAR_MAX_EXPERTS) return 0;
+    const qk::Matrix &operand = activation != QK_ACT_IDENTITY && grad_pre ? z : g;
+    return qk::plan_backward(g.rows, g.cols, (int)experts, activation, has_grad_bias != 0, grad_pre != nullptr,
+                             !qk::product_needs_aligned_rows(operand.rows, operand.ptr, operand.stride)).bytes;
 }
 
 }  // extern "C"

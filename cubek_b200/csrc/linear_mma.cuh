@@ -1,0 +1,492 @@
+// Products with quantized weights on the tensor cores: the weight is dequantized into shared memory on the way.
+//
+// The product is computed transposed, D^T [features, rows]: a tile has 128 features (256 for a pair of CTAs) as the
+// instruction's M and up to 256 rows of x as its N, so that a single row of x costs a tile of 16, not of 128.  Per step of 64
+// of the contraction, eight warps load codes and scales into registers (several steps ahead, the only way the
+// weight is read), turn them into f16 / bf16 and store them to the swizzled layout the instruction reads; one thread loads
+// the tile of x by bulk tensor copy; one thread issues the products; four warps take finished tiles from TMEM through the
+// epilogue while the next tile runs in the other half of TMEM.
+//   forward:  A [128 features = weight rows][64 columns], contraction contiguous (K-major)
+//   backward: A [128 features = weight columns][64 weight rows], features contiguous (MN-major): the codes are
+//             stored as they lie in memory and the instruction transposes
+// Few tiles: the contraction is split over a cluster of CTAs; each sends the others their share of its sums through
+// distributed shared memory and adds what it receives in rank order, so results do not depend on timing.
+#pragma once
+
+#include <atomic>
+
+#include "linear_kernels.cuh"
+#include "sm100.cuh"
+
+namespace qk {
+
+struct LinearMmaArgs {
+    LinearArgs a;
+    int tile_rows;    // rows of x per tile: a multiple of 16, at most 256
+    int stages;
+    int split;        // CTAs of a cluster that share a tile's contraction
+    int feat_tiles;
+    int tmem_columns;
+    int kblocks;      // steps of 64 of the contraction
+};
+
+constexpr int MMA_THREADS = 448;   // warps 0-3 epilogue, 4 loads x, 5 products, 6-13 weight
+constexpr int MMA_WEIGHT_WARPS = 8;
+constexpr int MMA_MAX_STAGES = 8;
+constexpr int A_BYTES = 128 * 64 * 2;
+constexpr int MMA_SMEM_LIMIT = 226 * 1024;   // dynamic; the barriers are static
+
+struct MmaTile {
+    int e, f0, r0, rows;
+};
+
+// Offsets of the tiles of each expert, in shared memory; experts == 1 needs none.
+struct MmaSchedule {
+    int total;          // tiles of all experts
+    int one_rows;       // a.offsets == nullptr
+    const int *prefix;  // [experts + 1] tiles of rows before expert e
+    const int *lo, *hi;
+};
+
+__device__ __forceinline__ MmaTile mma_tile(const LinearMmaArgs &m, const MmaSchedule &s, int t, int feats_per_tile)
+{
+    MmaTile r;
+    const int rt = t / m.feat_tiles;
+    r.f0 = (t - rt * m.feat_tiles) * feats_per_tile;
+    if (s.prefix == nullptr) {
+        r.e = 0;
+        r.r0 = rt * m.tile_rows;
+        r.rows = min(m.tile_rows, s.one_rows - r.r0);
+        return r;
+    }
+    int a = 0, b = m.a.experts;   // prefix[a] <= rt < prefix[b]
+    while (b - a > 1) {
+        const int mid = (a + b) / 2;
+        if (s.prefix[mid] <= rt) a = mid;
+        else b = mid;
+    }
+    r.e = a;
+    r.r0 = s.lo[a] + (rt - s.prefix[a]) * m.tile_rows;
+    r.rows = min(m.tile_rows, s.hi[a] - r.r0);
+    return r;
+}
+
+// 16 sums of one feature per lane, rows r .. r + 15 of the tile (valid: how many exist).
+template <int FDT>
+__device__ __forceinline__ void mma_store16(const LinearArgs &a, const float *v, int row, int valid, int f, float bias, float bias_even, float bias_odd)
+{
+    using F = typename ElemOf<FDT>::type;
+    if (a.pairs) {
+        // lanes 2i and 2i + 1 hold neighbouring features: the even one takes both of even rows, the odd one of odd rows
+        const int odd = threadIdx.x & 1, fe = f - odd;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            const float give = odd ? v[j] : v[j + 1];
+            const float got = __shfl_xor_sync(0xffffffffu, give, 1);
+            float z0 = (odd ? got : v[j]) + bias_even, z1 = (odd ? v[j + 1] : got) + bias_odd;
+            if (j + odd >= valid || f >= a.feats) continue;
+            const long long r = row + j + odd;
+            if (a.pre) *reinterpret_cast<uint32_t *>(static_cast<F *>(a.pre) + r * a.pre_stride + fe) = h2_pack<FDT>(z0, z1);
+            z0 = activate(a.act, z0);
+            z1 = activate(a.act, z1);
+            if (a.residual) {
+                const uint32_t q = *reinterpret_cast<const uint32_t *>(static_cast<const F *>(a.residual) + r * a.residual_stride + fe);
+                z0 += widen_lo<FDT>(q);
+                z1 += widen_hi<FDT>(q);
+            }
+            *reinterpret_cast<uint32_t *>(static_cast<F *>(a.out) + r * a.out_stride + fe) = h2_pack<FDT>(z0, z1);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < valid && f < a.feats) finish_one<FDT>(a, row + j, f, v[j], bias);
+    }
+}
+
+// CG: 1, or 2 for a pair of CTAs that works on one tile of 256 features with 2-CTA instructions.
+template <int KIND, int FDT, bool BWD, int CG>
+__global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid_constant__ CUtensorMap xmap, const LinearMmaArgs m)
+{
+    constexpr int AHEAD = CodeRun<KIND>::WORDS >= 8 ? 3 : 4;   // steps whose codes are in flight to registers
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[3 * MMA_MAX_STAGES + 5];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int gave_up;
+    const LinearArgs &a = m.a;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const int b_rows = m.tile_rows / CG;                        // rows of x this CTA loads
+    const uint32_t b_bytes = (uint32_t)b_rows * 128u, stage_bytes = A_BYTES + b_bytes;
+    int *table = reinterpret_cast<int *>(smem_raw + (base - smem_u32(smem_raw)) + m.stages * stage_bytes);
+    const uint32_t bar0 = smem_u32(bars);
+    const auto full_x = [&](int s) { return bar0 + 8u * s; };
+    const auto full_w = [&](int s) { return bar0 + 8u * (MMA_MAX_STAGES + s); };
+    const auto empty = [&](int s) { return bar0 + 8u * (2 * MMA_MAX_STAGES + s); };
+    const auto acc_full = [&](int b) { return bar0 + 8u * (3 * MMA_MAX_STAGES + b); };
+    const auto acc_empty = [&](int b) { return bar0 + 8u * (3 * MMA_MAX_STAGES + 2 + b); };
+    const uint32_t drained = bar0 + 8u * (3 * MMA_MAX_STAGES + 4);
+    const uint32_t rank = (CG == 2 || m.split > 1) ? cluster_rank() : 0u;
+    const bool leader = CG == 1 || rank == 0;
+
+    if (threadIdx.x == 0) {
+        gave_up = 0;
+        for (int s = 0; s < MMA_MAX_STAGES; ++s) {
+            mbar_init(full_x(s), 1);
+            mbar_init(full_w(s), MMA_WEIGHT_WARPS * CG);
+            mbar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(acc_full(b), 1);
+            mbar_init(acc_empty(b), 4 * CG);
+        }
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 5) tmem_alloc<CG>(smem_u32(&tmem_slot), m.tmem_columns);
+    pdl_entry();
+
+    MmaSchedule sched;
+    sched.prefix = nullptr;
+    sched.one_rows = a.rows;
+    if (a.offsets != nullptr) {
+        int *prefix = table, *lo = table + a.experts + 1, *hi = lo + a.experts;
+        for (int e = threadIdx.x; e < a.experts; e += MMA_THREADS) {
+            int l, h;
+            expert_rows(a, e, l, h);
+            lo[e] = l;
+            hi[e] = h;
+        }
+        __syncthreads();
+        if (warp == 0) {   // running sum of the experts' tiles of rows
+            int sum = 0;
+            for (int e0 = 0; e0 < a.experts; e0 += 32) {
+                const int e = e0 + lane;
+                int n = e < a.experts ? (hi[e] - lo[e] + m.tile_rows - 1) / m.tile_rows : 0;
+#pragma unroll
+                for (int d = 1; d < 32; d *= 2) {
+                    const int up = __shfl_up_sync(0xffffffffu, n, d);
+                    if (lane >= d) n += up;
+                }
+                if (e < a.experts) prefix[e + 1] = sum + n;
+                sum += __shfl_sync(0xffffffffu, n, 31);
+            }
+            if (lane == 0) prefix[0] = 0;
+        }
+        __syncthreads();
+        sched.prefix = prefix;
+        sched.lo = lo;
+        sched.hi = hi;
+        sched.total = prefix[a.experts] * m.feat_tiles;
+    } else {
+        sched.total = (a.rows + m.tile_rows - 1) / m.tile_rows * m.feat_tiles;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (CG == 2 || m.split > 1) cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    // Every wait is bounded: a thread that gives up says so to the others of its CTA and to the host, and from then on
+    // waits for nothing and starts nothing.
+    bool dead = false;
+    const auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (!dead && !mbar_wait(bar, parity, &gave_up)) {
+            dead = true;
+            *(volatile int *)&gave_up = 1;
+            atomicExch(a.error_flag, 1);
+        }
+    };
+
+    const int members = CG * m.split;
+    const int first = blockIdx.x / members, step = gridDim.x / members;
+    const int kb0 = CG == 1 ? (int)((long long)m.kblocks * rank / m.split) : 0;
+    const int kb1 = CG == 1 ? (int)((long long)m.kblocks * (rank + 1) / m.split) : m.kblocks;
+    constexpr int TILE_FEATS = 128 * CG;
+    int stage = 0, phase = 0;
+    const auto next_stage = [&] {
+        if (++stage == m.stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    };
+    // With a split contraction the CTAs of a cluster meet twice per tile: all sums are ready (the stages are free and
+    // take the exchange), all shares have arrived; then the CTA's own warps meet before the stages are filled again.
+    const auto meet = [&] {
+        __syncwarp();
+        cluster_sync();
+    };
+    const auto meet_cta = [&] { asm volatile("bar.sync 1, %0;" ::"n"(MMA_THREADS) : "memory"); };
+
+    if (warp == 4) {
+        // ---- tile of x ----------------------------------------------------------------------------------
+        int started = 0;
+        for (int t = first; t < sched.total; t += step) {
+            const MmaTile tile = mma_tile(m, sched, t, TILE_FEATS);
+            if (lane == 0) {
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    wait(empty(stage), phase ^ 1);
+                    if (dead) break;
+                    const uint32_t dst = base + stage * stage_bytes + A_BYTES;
+                    if (CG == 1) {
+                        mbar_expect_tx(full_x(stage), b_bytes);
+                        tma_load_2d(dst, &xmap, kb * 64, tile.r0, full_x(stage));
+                    } else {
+                        if (leader) mbar_expect_tx(full_x(stage), 2 * b_bytes);
+                        tma_load_2d_pair(dst, &xmap, kb * 64, tile.r0 + (int)rank * b_rows, full_x(stage));
+                    }
+                    ++started;
+                    next_stage();
+                }
+            }
+            if (m.split > 1) {
+                meet();
+                meet();
+                meet_cta();
+            }
+        }
+        if (dead && leader) {   // copies in flight still write to this CTA's memory: wait for them, again within a limit
+            for (int i = min(started, m.stages); i > 0; --i) {
+                stage = stage == 0 ? m.stages - 1 : stage - 1;
+                if (stage == m.stages - 1) phase ^= 1;
+                mbar_wait(full_x(stage), phase, nullptr);
+            }
+        }
+    } else if (warp == 5) {
+        // ---- products -----------------------------------------------------------------------------------
+        const uint32_t idesc = instr_desc(FDT == QK_BF16, BWD, 128 * CG, m.tile_rows);
+        int buf = 0, buf_phase = 0;
+        for (int t = first; t < sched.total; t += step) {
+            if (lane == 0 && leader && kb0 < kb1) {
+                wait(acc_empty(buf), buf_phase ^ 1);
+                tc_fence_after();
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    wait(full_x(stage), phase);
+                    wait(full_w(stage), phase);
+                    if (dead) break;
+                    tc_fence_after();
+                    const uint32_t sa = base + stage * stage_bytes, sb = sa + A_BYTES;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // K-major: 16 steps are 32 bytes of a swizzled row.  MN-major: two groups of 8 rows of 128 bytes.
+                        const uint64_t da = BWD ? smem_desc(sa + i * 2048, 8192, 1024) : smem_desc(sa + i * 32, 16, 1024);
+                        const uint64_t db = smem_desc(sb + i * 32, 16, 1024);
+                        mma_f16<CG>(tmem + buf * m.tile_rows, da, db, idesc, kb > kb0 || i > 0);
+                    }
+                    mma_commit<CG>(empty(stage));
+                    next_stage();
+                }
+                mma_commit<CG>(acc_full(buf));
+                buf ^= 1;
+                if (buf == 0) buf_phase ^= 1;
+            }
+            if (m.split > 1) {
+                meet();
+                meet();
+                meet_cta();
+            }
+        }
+        if (lane == 0 && leader) {   // nothing may be in flight to TMEM when it is freed
+            mma_commit<CG>(drained);
+            mbar_wait(drained, 0, nullptr);
+        }
+        __syncwarp();
+    } else if (warp >= 6) {
+        // ---- weight -------------------------------------------------------------------------------------
+        // A thread's 32 codes of a step: 8 neighbouring lanes store to 8 different 16-byte columns of the swizzle.
+        const int id = threadIdx.x - 6 * 32, half = BWD ? id / 128 : 0;
+        const int r = BWD ? (id / 2) % 64 : id / 2, c = (id & 1) * 4;
+        const uint32_t mine = BWD ? half * 8192 + r * 128 : r * 128;
+        CodeRun<KIND> run[AHEAD];
+        int lt = first, lkb = kb0;   // the step that is loaded next
+        MmaTile ltile = {};
+        if (lt < sched.total) ltile = mma_tile(m, sched, lt, TILE_FEATS);
+        const auto load_next = [&](CodeRun<KIND> &q) {
+            if (lt >= sched.total) return;
+            const int f = ltile.f0 + (CG == 2 ? (int)rank * 128 : 0);
+            const int row = BWD ? lkb * 64 + r : f + r, col = BWD ? f + half * 64 + (id & 1) * 32 : lkb * 64 + (id & 1) * 32;
+            load_code_run<KIND>(a, q, ltile.e, row, col);
+            if (++lkb >= kb1) {
+                lkb = kb0;
+                lt += step;
+                if (lt < sched.total) ltile = mma_tile(m, sched, lt, TILE_FEATS);
+            }
+        };
+        if (kb0 < kb1) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) load_next(run[i]);
+            int t = first, kb = kb0;
+            while (t < sched.total) {
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    if (t >= sched.total) break;
+                    uint32_t o[16];
+                    decode_code_run<KIND, FDT>(a, run[i], o);
+                    load_next(run[i]);
+                    wait(empty(stage), phase ^ 1);
+                    const uint32_t dst = base + stage * stage_bytes + mine;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (uint32_t)(((c + j) ^ (r & 7)) * 16)), "r"(o[4 * j]),
+                                     "r"(o[4 * j + 1]), "r"(o[4 * j + 2]), "r"(o[4 * j + 3])
+                                     : "memory");
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0 && !dead) {
+                        if (CG == 1) mbar_arrive(full_w(stage));
+                        else mbar_arrive_cluster(full_w(stage), 0);
+                    }
+                    next_stage();
+                    if (++kb >= kb1) {
+                        kb = kb0;
+                        t += step;
+                        if (m.split > 1) {
+                            meet();
+                            meet();
+                            meet_cta();
+                        }
+                    }
+                }
+            }
+        } else if (m.split > 1) {
+            for (int t = first; t < sched.total; t += step) {
+                meet();
+                meet();
+                meet_cta();
+            }
+        }
+    } else {
+        // ---- epilogue -----------------------------------------------------------------------------------
+        int buf = 0, buf_phase = 0;
+        for (int t = first; t < sched.total; t += step) {
+            const MmaTile tile = mma_tile(m, sched, t, TILE_FEATS);
+            const int f = tile.f0 + (CG == 2 ? (int)rank * 128 : 0) + (int)threadIdx.x;
+            const float bias = load_bias<FDT>(a, tile.e, f);
+            const float bias_even = __shfl_sync(0xffffffffu, bias, lane & ~1), bias_odd = __shfl_sync(0xffffffffu, bias, lane | 1);
+            const uint32_t from = tmem + ((uint32_t)warp << 21) + buf * m.tile_rows;   // lane 32 * warp
+            const bool sums = kb0 < kb1;
+            if (sums) {
+                wait(acc_full(buf), buf_phase);
+                dead = __any_sync(0xffffffffu, dead);
+                tc_fence_after();
+            }
+            if (m.split == 1) {
+                for (int r = 0; r < tile.rows; r += 16) {
+                    float v[16];
+                    if (sums) {
+                        tmem_load16(from + r, v);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+                    }
+                    if (!dead) mma_store16<FDT>(a, v, tile.r0 + r, tile.rows - r, f, bias, bias_even, bias_odd);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0 && sums && !dead) {
+                    if (CG == 1) mbar_arrive(acc_empty(buf));
+                    else mbar_arrive_cluster(acc_empty(buf), 0);
+                }
+            } else {
+                // rows of the tile in shares of `share`; share i is finished by CTA i
+                const int share = m.tile_rows / m.split;
+                meet();
+                for (int r = 0; r < m.tile_rows; r += 16) {
+                    float v[16];
+                    if (sums) {
+                        tmem_load16(from + r, v);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int owner = (r + i) / share, at = (r + i) - owner * share;
+                        if (r + i < tile.rows) st_cluster_f32(cluster_map(base + ((rank * share + at) * 128 + threadIdx.x) * 4, owner), v[i]);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0 && sums && !dead) mbar_arrive(acc_empty(buf));
+                meet();
+                const float *got = reinterpret_cast<const float *>(smem_raw + (base - smem_u32(smem_raw)));
+                const int r0 = (int)rank * share;
+                for (int r = 0; r < share && r0 + r < tile.rows; r += 16) {
+                    float v[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        v[i] = 0.0f;
+                        if (r + i < share && r0 + r + i < tile.rows)
+                            for (int s = 0; s < m.split; ++s) v[i] += got[(s * share + r + i) * 128 + threadIdx.x];
+                    }
+                    if (!dead) mma_store16<FDT>(a, v, tile.r0 + r0 + r, min(share - r, tile.rows - r0 - r), f, bias, bias_even, bias_odd);
+                }
+                fence_async_shared();   // what was read here is written by bulk copies next
+                meet_cta();
+            }
+            if (sums) {
+                buf ^= 1;
+                if (buf == 0) buf_phase ^= 1;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (CG == 2 || m.split > 1) cluster_sync();   // a CTA's memory stays until the others have stopped using it
+    if (warp == 5) {
+        tc_fence_after();
+        tmem_free<CG>(tmem, m.tmem_columns);
+    }
+}
+
+// ---- launch -------------------------------------------------------------------------------------------------
+template <int KIND, int FDT, bool BWD, int CG>
+static cudaError_t launch_mma_one(const CUtensorMap &map, const LinearMmaArgs &m, int grid, size_t smem, const LaunchCfg &cfg, cudaStream_t stream)
+{
+    static std::atomic<unsigned long long> ready{0};   // devices whose shared-memory limit of this kernel is raised
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {
+        e = cudaFuncSetAttribute(linear_mma_kernel<KIND, FDT, BWD, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, MMA_SMEM_LIMIT);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((unsigned)grid);
+    c.blockDim = dim3(MMA_THREADS);
+    c.dynamicSmemBytes = smem;
+    c.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (cfg.pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (CG * m.split > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = CG * m.split;
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
+    c.attrs = attr;
+    c.numAttrs = n;
+    return cudaLaunchKernelEx(&c, linear_mma_kernel<KIND, FDT, BWD, CG>, map, m);
+}
+
+template <int FDT, bool BWD, int CG>
+static cudaError_t launch_mma_kind(int kind, const CUtensorMap &map, const LinearMmaArgs &m, int grid, size_t smem, const LaunchCfg &cfg,
+                                   cudaStream_t stream)
+{
+    switch (kind) {
+    case KIND_PACK8:   // bytes either way
+    case KIND_I8: return launch_mma_one<KIND_I8, FDT, BWD, CG>(map, m, grid, smem, cfg, stream);
+    case KIND_PACK4: return launch_mma_one<KIND_PACK4, FDT, BWD, CG>(map, m, grid, smem, cfg, stream);
+    case KIND_PACK2: return launch_mma_one<KIND_PACK2, FDT, BWD, CG>(map, m, grid, smem, cfg, stream);
+    case KIND_E2M1: return launch_mma_one<KIND_E2M1, FDT, BWD, CG>(map, m, grid, smem, cfg, stream);
+    case KIND_E4M3: return launch_mma_one<KIND_E4M3, FDT, BWD, CG>(map, m, grid, smem, cfg, stream);
+    case KIND_E5M2: return launch_mma_one<KIND_E5M2, FDT, BWD, CG>(map, m, grid, smem, cfg, stream);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace qk

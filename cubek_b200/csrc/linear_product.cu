@@ -1,0 +1,90 @@
+// Which kernel a product with a quantized weight takes, and its launch.
+#include "host_checks.cuh"
+#include "linear_backward.cuh"
+#include "linear_mma.cuh"
+
+namespace qk {
+
+cudaError_t launch_mma_forward_f16(int, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
+cudaError_t launch_mma_forward_bf16(int, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
+cudaError_t launch_mma_backward_f16(int, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
+cudaError_t launch_mma_backward_bf16(int, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
+
+bool product_needs_aligned_rows(long long rows, const void *x, long long stride)
+{
+    return reinterpret_cast<uintptr_t>(x) % 16 != 0 || (rows > 1 && stride % 8 != 0);
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                 const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encode_tiled()
+{
+    static std::atomic<void *> found{nullptr};
+    void *p = found.load(std::memory_order_acquire);
+    if (!p) {
+        cudaDriverEntryPointQueryResult how;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &how) != cudaSuccess ||
+            how != cudaDriverEntryPointSuccess)
+            return nullptr;
+        found.store(p, std::memory_order_release);
+    }
+    return reinterpret_cast<EncodeTiled>(p);
+}
+
+static int round_up(int v, int to) { return (v + to - 1) / to * to; }
+
+static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
+{
+    LinearMmaArgs m = {};
+    m.a = a;
+    const bool grouped = a.offsets != nullptr;
+    long long row_tiles;
+    if (!grouped) {
+        const int tiles = (a.rows + 255) / 256;
+        m.tile_rows = round_up((a.rows + tiles - 1) / tiles, 16);
+        row_tiles = tiles;
+    } else {
+        const int average = a.rows / a.experts;
+        m.tile_rows = average >= 128 ? 256 : round_up(2 * average + 1, 16);
+        row_tiles = a.rows / m.tile_rows + (a.experts < a.rows ? a.experts : a.rows);   // at most
+    }
+    m.feat_tiles = (a.feats + 127) / 128;
+    m.kblocks = (a.contraction + 63) / 64;
+    const long long tiles = row_tiles * m.feat_tiles;
+    if (tiles >= (1ll << 31)) return cudaErrorInvalidConfiguration;
+    m.split = 1;
+    while (m.split < 8 && tiles * m.split * 2 <= cfg.sm_count && m.kblocks / (m.split * 2) >= 4) m.split *= 2;
+    const int stage_bytes = A_BYTES + m.tile_rows * 128;
+    const int table = grouped ? (3 * a.experts + 1) * 4 : 0;
+    m.stages = (MMA_SMEM_LIMIT - 1024 - table) / stage_bytes;
+    if (m.stages > MMA_MAX_STAGES) m.stages = MMA_MAX_STAGES;
+    m.tmem_columns = 32;
+    while (m.tmem_columns < 2 * m.tile_rows) m.tmem_columns *= 2;
+    const long long clusters = cfg.sm_count / m.split;
+    const int grid = (int)(tiles < clusters ? tiles : clusters) * m.split;
+    const size_t smem = 1024 + (size_t)m.stages * stage_bytes + table;
+
+    CUtensorMap map = {};
+    if (m.kblocks > 0) {
+        const EncodeTiled encode = encode_tiled();
+        if (!encode) return cudaErrorNotSupported;
+        const cuuint64_t dims[2] = {(cuuint64_t)a.contraction, (cuuint64_t)a.rows};
+        const cuuint64_t strides[1] = {(cuuint64_t)(a.rows > 1 ? a.x_stride * 2 : round_up(a.contraction, 8) * 2ll)};
+        const cuuint32_t box[2] = {64, (cuuint32_t)m.tile_rows}, ones[2] = {1, 1};
+        const CUresult r = encode(&map, fdt == QK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(a.x), dims,
+                                  strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return cudaErrorInvalidValue;
+    }
+    if (fdt == QK_F16)
+        return backward ? launch_mma_backward_f16(kind, map, m, grid, smem, cfg, stream) : launch_mma_forward_f16(kind, map, m, grid, smem, cfg, stream);
+    return backward ? launch_mma_backward_bf16(kind, map, m, grid, smem, cfg, stream) : launch_mma_forward_bf16(kind, map, m, grid, smem, cfg, stream);
+}
+
+cudaError_t launch_linear_product(int fdt, int kind, bool backward, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
+{
+    return launch_mma(fdt, kind, backward, a, cfg, stream);
+}
+
+}  // namespace qk

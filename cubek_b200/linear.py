@@ -31,11 +31,13 @@ def workspace_bytes(input: TensorHandleRef, weight: MatmulInputHandleRef, dtype:
 
 
 def backward_workspace_bytes(grad_output: TensorHandleRef, weight: MatmulInputHandleRef, dtype: ElemType,
-                             activation: Activation = Activation.Identity, bias: bool = False, grad_pre: bool = False) -> int:
-    """Device workspace of the backward call; ``bias`` and ``grad_pre`` say whether those gradients are asked for."""
+                             activation: Activation = Activation.Identity, bias: bool = False,
+                             grad_pre: TensorHandleRef | None = None) -> int:
+    """Device workspace of the backward call; ``bias``: ``grad_bias`` is asked for; ``grad_pre``: what the call gets there."""
     tg, tv = _ffi.c_tensors(grad_output, weight.data)
+    keep, pre = _ffi.optional(grad_pre)
     return _ffi.lib().qk_linear_backward_workspace_bytes(tg.ref(), tv.ref(), _ffi.c_scheme(weight.scheme), int(activation), int(bias),
-                                                         int(grad_pre), int(dtype))
+                                                         pre, int(dtype))
 
 
 class _Call:

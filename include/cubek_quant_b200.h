@@ -341,11 +341,13 @@ int qk_grouped_linear_backward(const QkTensor *grad_output, const QkTensor *offs
                                const QkTensor *grad_bias, const QkTensor *grad_pre, int dtype, void *workspace, size_t workspace_bytes,
                                void *stream);
 
-/* Device workspace of these calls (16-byte aligned; `values` of rank 3 for the grouped forms).  It needs no
- * initialisation and holds nothing between calls; calls that may overlap need one each. */
+/* Device workspace of these calls for tensors at these addresses (16-byte aligned; `values` of rank 3 for the grouped
+ * forms).  Forward: none where the rows of x start on 16 bytes, else a copy of x whose rows do.  Backward: dz
+ * where grad_pre (NULL: not asked for) does not take it, and partial bias sums.  It needs no initialisation and holds
+ * nothing between calls; calls that may overlap need one each. */
 size_t qk_linear_workspace_bytes(const QkTensor *input, const QkTensor *values, const QkScheme *scheme, int dtype);
 size_t qk_linear_backward_workspace_bytes(const QkTensor *grad_output, const QkTensor *values, const QkScheme *scheme, int activation,
-                                          int has_grad_bias, int has_grad_pre, int dtype);
+                                          int has_grad_bias, const QkTensor *grad_pre, int dtype);
 
 const char *qk_strerror(int status);
 const char *qk_version(void);

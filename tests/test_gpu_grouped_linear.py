@@ -32,7 +32,7 @@ def run(w: Weight, counts, rows, first=0, act=Activation.Identity, bias=False, r
     ws = workspace(grouped_linear.workspace_bytes(H(x), handle, elem))
     grouped_linear.launch(client, H(x), H(off), handle, H(y), elem, bias=opt(b), residual=opt(r), activation=act, pre=H(pre), workspace=H(ws))
     g = randn((rows, n), elem, seed + 3)
-    ws = workspace(grouped_linear.backward_workspace_bytes(H(g), handle, elem, activation=act, bias=True, grad_pre=True))
+    ws = workspace(grouped_linear.backward_workspace_bytes(H(g), handle, elem, activation=act, bias=True, grad_pre=H(gp)))
     grouped_linear.launch_backward(client, H(g), H(off), handle, H(gx), elem, pre=H(pre), activation=act, grad_bias=H(gb), grad_pre=H(gp),
                                    workspace=H(ws))
     # the same through the staged dz

@@ -45,7 +45,7 @@ def backward(w: Weight, g, pre=None, act=Activation.Identity, bias=True, keep=Tr
     gp = filled(g.shape, w.elem) if keep else None
     handle = handle or w.handle()
     opt = lambda t: None if t is None else H(t)  # noqa: E731
-    ws = workspace(linear.backward_workspace_bytes(H(g), handle, w.elem, activation=act, bias=bias, grad_pre=keep))
+    ws = workspace(linear.backward_workspace_bytes(H(g), handle, w.elem, activation=act, bias=bias, grad_pre=opt(gp)))
     linear.launch_backward(ComputeClient.current(), H(g), handle, H(gx), w.elem, pre=opt(pre), activation=act, grad_bias=opt(gb),
                            grad_pre=opt(gp), workspace=H(ws))
     return gx, gb, gp

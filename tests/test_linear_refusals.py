@@ -133,7 +133,7 @@ def test_null_arguments():
         args[i] = None
         assert lib.qk_linear_backward(*args) == _ffi.QK_ERR_NULL
     assert lib.qk_grouped_linear(x.ref(), None, v.ref(), p.ref(), s, None, None, 0, x.ref(), None, int(BF), None, 0, None) != _ffi.QK_OK
-    assert lib.qk_linear_backward_workspace_bytes(None, v.ref(), s, 0, 0, 0, int(BF)) == 0
+    assert lib.qk_linear_backward_workspace_bytes(None, v.ref(), s, 0, 0, None, int(BF)) == 0
     assert lib.qk_linear_workspace_bytes(None, v.ref(), s, int(BF)) == 0
 
 
@@ -152,7 +152,7 @@ def test_workspace_sizes():
     assert plain == 0
     staged = linear.backward_workspace_bytes(g, w, BF, activation=Activation.Silu)
     assert staged >= 1000 * 512 * 2
-    assert linear.backward_workspace_bytes(g, w, BF, activation=Activation.Silu, grad_pre=True) == 0
+    assert linear.backward_workspace_bytes(g, w, BF, activation=Activation.Silu, grad_pre=g) == 0
     assert linear.backward_workspace_bytes(g, w, BF, bias=True) % 256 == 0
     handle = MatmulInputHandleRef.quantized(fake((3, 512, 32), 4), fake((3, 512, 8), 4), (3, 512, 256), Q4)
     assert grouped_linear.backward_workspace_bytes(g, handle, BF, activation=Activation.Silu) >= 1000 * 512 * 2
