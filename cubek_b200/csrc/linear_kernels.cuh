@@ -100,20 +100,41 @@ __device__ __forceinline__ float activation_slope(int act, float z)
 }
 
 // ---- weights ----------------------------------------------------------------------------------------
-// A run of 32 consecutive codes of one weight row as it lies in memory, with its scales as stored.
+// A run of 32 consecutive codes of one weight row, at a column that is a multiple of 32, with its scales as stored.
 template <int KIND> struct CodeRun {
     static constexpr int BITS = kind_bits(KIND);
     static constexpr int WORDS = BITS;  // 32 codes of BITS bits
     uint32_t w[WORDS];
-    uint32_t s[4];  // raw scale of each 8 codes (only s[0] with scale32)
-    int valid;      // codes of the run that exist (0 .. 32); the others are zero bits
+    uint32_t s[4];  // raw scale of each 8 codes (with scale32 only s[0])
 };
 
-__device__ __forceinline__ uint32_t load_scale_raw(const LinearArgs &a, long long i)
+// A weight row: its codes and its scales.
+struct CodeRow {
+    const uint8_t *codes;
+    long long scale;  // index of its first scale
+    int exists;
+};
+
+__device__ __forceinline__ CodeRow code_row(const LinearArgs &a, int e, int row)
 {
-    return a.param == QK_F32 ? __ldg(static_cast<const uint32_t *>(a.scales) + i)
-                             : (uint32_t)__ldg(static_cast<const unsigned short *>(a.scales) + i);
+    CodeRow c;
+    c.codes = a.codes + e * a.code_expert + row * a.code_row;
+    c.scale = (long long)(e / a.be) * a.scale_expert + (long long)fastdiv((unsigned)row, a.bn) * a.scale_row;
+    c.exists = row < a.n;
+    return c;
 }
+
+__device__ __forceinline__ int codes_left(const LinearArgs &a, int col)
+{
+    const int left = a.k - col;
+    return left < 0 ? 0 : left > 32 ? 32 : left;
+}
+
+__device__ __forceinline__ long long scale_index(const LinearArgs &a, const CodeRow &row, int col)
+{
+    return row.scale + (long long)fastdiv((unsigned)col, a.bk) * a.scale_col;
+}
+
 // RN_F(scale) as f32.
 template <int FDT> __device__ __forceinline__ float scale_value(const LinearArgs &a, uint32_t raw)
 {
@@ -123,89 +144,146 @@ template <int FDT> __device__ __forceinline__ float scale_value(const LinearArgs
     return round_to<FDT>(s);
 }
 
-// Codes row, col .. col + 31 of expert e; row and col may lie past the weight.  col is a multiple of 32.
-template <int KIND> __device__ __forceinline__ void load_code_run(const LinearArgs &a, CodeRun<KIND> &r, int e, int row, int col)
+// The run as 16 registers of packed F x2, in element order; codes past `valid` are +0 whatever the scale is.
+// WHOLE: one scale and all 32 codes exist.
+template <int KIND, int FDT, bool WHOLE> __device__ __forceinline__ void decode_code_run(const LinearArgs &a, const CodeRun<KIND> &r, int valid, uint32_t *o)
 {
-    constexpr int BITS = CodeRun<KIND>::BITS, WORDS = CodeRun<KIND>::WORDS;
-    int valid = row < a.n ? a.k - col : 0;
-    valid = valid < 0 ? 0 : valid > 32 ? 32 : valid;
-    r.valid = valid;
+    constexpr int WORDS = CodeRun<KIND>::WORDS, EPW = kind_elems_per_u32(KIND);
+    float s[4];
+    s[0] = scale_value<FDT>(a, r.s[0]);
+    s[1] = s[2] = s[3] = s[0];
+    if (!WHOLE && !a.scale32) {
 #pragma unroll
-    for (int i = 0; i < WORDS; ++i) r.w[i] = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.s[i] = 0;
-    if (valid == 0) return;
-    const uint8_t *p = a.codes + e * a.code_expert + row * a.code_row + (long long)col * BITS / 8;
-    const int bytes = (valid * BITS + 7) / 8;
-    if (a.code_align == 16 && valid == 32) {
-        if constexpr (WORDS == 2) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-            r.w[0] = v.x;
-            r.w[1] = v.y;
-        } else {
-#pragma unroll
-            for (int i = 0; i < WORDS / 4; ++i) {
-                const Vec16 v = ldg128_stream(p + 16 * i);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) r.w[4 * i + j] = v.w[j];
-            }
-        }
-    } else if (a.code_align >= 4) {
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) {
-            if (4 * i + 4 <= bytes) {
-                r.w[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
-            } else {
-                for (int j = 4 * i; j < bytes; ++j) r.w[i] |= (uint32_t)__ldg(p + j) << (8 * (j - 4 * i));
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (4 * i + j < bytes) r.w[i] |= (uint32_t)__ldg(p + 4 * i + j) << (8 * j);
+        for (int g = 1; g < 4; ++g) s[g] = scale_value<FDT>(a, r.s[g]);
     }
-    const long long s0 = (long long)(e / a.be) * a.scale_expert + (long long)fastdiv((unsigned)row, a.bn) * a.scale_row;
-    if (a.scale32) {
-        r.s[0] = load_scale_raw(a, s0 + (long long)fastdiv((unsigned)col, a.bk) * a.scale_col);
-    } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (8 * i < valid) r.s[i] = load_scale_raw(a, s0 + (long long)fastdiv((unsigned)(col + 8 * i), a.bk) * a.scale_col);
+    for (int i = 0; i < WORDS; ++i) {   // 16 codes of a word: their blocks are multiples of 16 codes
+        const float sc = s[i * EPW / 8];
+        dequant_word<FDT, KIND>(r.w[i], sc, h2_pack<FDT>(sc, sc), o + i * EPW / 2);
+    }
+    if (!WHOLE && valid < 32) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (2 * i >= valid) o[i] = 0;
+            else if (2 * i + 1 >= valid) o[i] &= 0xffffu;
+        }
     }
 }
 
-// The run as 16 registers of packed F x2, in element order; what lies past the weight is +0 whatever the scale is.
-template <int KIND, int FDT> __device__ __forceinline__ void decode_code_run(const LinearArgs &a, const CodeRun<KIND> &r, uint32_t *o)
+// Runs on their way from memory: a thread copies its own ones to its own places in shared memory by asynchronous copies
+// of 16, 8 or 4 bytes, several steps ahead, and nothing but the thread itself waits for them.  (Held in registers instead, the
+// unrolled copies of the loop body for each step in flight cost more instruction fetches than the arithmetic: 1600 cycles
+// a step of 128 x 64 codes, 900 with nothing to do.)
+template <int KIND> struct StagedRuns {
+    static constexpr int WORDS = CodeRun<KIND>::WORDS;
+    static constexpr int AHEAD = WORDS >= 8 ? 3 : 4;
+    __host__ __device__ static int slot_bytes(int threads, int scale32) { return threads * (WORDS * 4 + (scale32 ? 4 : 16)); }
+};
+
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void *src, int bytes)
 {
-    constexpr int WORDS = CodeRun<KIND>::WORDS, EPW = kind_elems_per_u32(KIND);
-    if (a.scale32) {
-        const float s = scale_value<FDT>(a, r.s[0]);
-        const uint32_t s2 = h2_pack<FDT>(s, s);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_async8(uint32_t dst, const void *src, int bytes)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_async4(uint32_t dst, const void *src, int bytes)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// Starts the copy of codes col .. col + 31 into the slot at shared address `slot` (thread `id` of `threads`); what lies past
+// the weight becomes zero bits.  Scales of 16 bits are copied with the aligned word that holds them.
+template <int KIND>
+__device__ __forceinline__ void stage_code_run(const LinearArgs &a, uint32_t slot, int id, int threads, const CodeRow &row, int col)
+{
+    constexpr int BITS = CodeRun<KIND>::BITS, WORDS = CodeRun<KIND>::WORDS;
+    const int valid = row.exists ? codes_left(a, col) : 0;
+    const int bytes = (valid * BITS + 7) / 8;
+    const uint8_t *p = valid ? row.codes + (long long)col * BITS / 8 : a.codes;
+    if (a.code_align == 16) {
+        if constexpr (WORDS == 2) {
+            copy_async8(slot + id * 8, p, bytes);
+        } else {
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) dequant_word<FDT, KIND>(r.w[i], s, s2, o + i * EPW / 2);
-    } else if constexpr (EPW <= 8) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float s = scale_value<FDT>(a, r.s[g]);
-            const uint32_t s2 = h2_pack<FDT>(s, s);
-#pragma unroll
-            for (int i = g * WORDS / 4; i < (g + 1) * WORDS / 4; ++i) dequant_word<FDT, KIND>(r.w[i], s, s2, o + i * EPW / 2);
+            for (int i = 0; i < WORDS / 4; ++i) {
+                const int left = bytes - 16 * i;
+                copy_async16(slot + (i * threads + id) * 16, left > 0 ? p + 16 * i : a.codes, left < 0 ? 0 : left > 16 ? 16 : left);
+            }
         }
-    } else {  // 16 codes a word: their blocks are multiples of 16 codes
-#pragma unroll
+    } else {
+#pragma unroll 1
         for (int i = 0; i < WORDS; ++i) {
-            const float s = scale_value<FDT>(a, r.s[2 * i]);
-            dequant_word<FDT, KIND>(r.w[i], s, h2_pack<FDT>(s, s), o + i * EPW / 2);
+            const uint32_t dst = WORDS == 2 ? slot + id * 8 + i * 4 : slot + ((i / 4) * threads + id) * 16 + (i % 4) * 4;
+            const int left = bytes - 4 * i < 0 ? 0 : bytes - 4 * i > 4 ? 4 : bytes - 4 * i;
+            if (a.code_align >= 4) {
+                copy_async4(dst, left > 0 ? p + 4 * i : reinterpret_cast<const uint8_t *>((uintptr_t)a.codes & ~(uintptr_t)3), left);
+            } else {
+                uint32_t v = 0;
+                for (int j = 0; j < left; ++j) v |= (uint32_t)__ldg(p + 4 * i + j) << (8 * j);
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(v) : "memory");
+            }
         }
     }
-    if (r.valid < 32) {
+    const uint32_t scales = slot + threads * WORDS * 4 + id * 4;
+    const int count = a.scale32 ? 1 : 4;
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+        const bool take = 8 * i < valid;
+        const long long at = take ? scale_index(a, row, col + 8 * i) : 0;
+        const uintptr_t q = reinterpret_cast<uintptr_t>(a.scales) + (a.param == QK_F32 ? at * 4 : at * 2);
+        copy_async4(scales + i * threads * 4, reinterpret_cast<const void *>(q & ~(uintptr_t)3), take ? 4 : 0);
+    }
+}
+
+// The same where every run is complete or lies wholly past the weight, starts on 16 bytes (8 for 2-bit codes) and has one scale.
+template <int KIND>
+__device__ __forceinline__ void stage_whole_run(const LinearArgs &a, uint32_t slot, int id, int threads, const CodeRow &row, int col)
+{
+    constexpr int BITS = CodeRun<KIND>::BITS, WORDS = CodeRun<KIND>::WORDS;
+    const bool ok = row.exists && col < a.k;
+    const uint8_t *p = ok ? row.codes + (col * BITS) / 8 : a.codes;
+    if constexpr (WORDS == 2) {
+        copy_async8(slot + id * 8, p, ok ? 8 : 0);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if (2 * i >= r.valid) o[i] = 0;
-            else if (2 * i + 1 >= r.valid) o[i] &= 0xffffu;
+        for (int i = 0; i < WORDS / 4; ++i) copy_async16(slot + (i * threads + id) * 16, p + 16 * i, ok ? 16 : 0);
+    }
+    const long long at = ok ? scale_index(a, row, col) : 0;
+    const uintptr_t q = reinterpret_cast<uintptr_t>(a.scales) + (a.param == QK_F32 ? at * 4 : at * 2);
+    copy_async4(slot + threads * WORDS * 4 + id * 4, reinterpret_cast<const void *>(q & ~(uintptr_t)3), ok ? 4 : 0);
+}
+
+// The staged run, once its copies have arrived.
+template <int KIND, bool WHOLE>
+__device__ __forceinline__ void take_code_run(const LinearArgs &a, CodeRun<KIND> &r, uint32_t slot, int id, int threads, const CodeRow &row, int col)
+{
+    constexpr int WORDS = CodeRun<KIND>::WORDS;
+    if constexpr (WORDS == 2) {
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "r"(slot + id * 8) : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < WORDS; i += 4)
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(r.w[i]), "=r"(r.w[i + 1]), "=r"(r.w[i + 2]), "=r"(r.w[i + 3])
+                         : "r"(slot + (i / 4 * threads + id) * 16)
+                         : "memory");
+    }
+    const uint32_t scales = slot + threads * WORDS * 4 + id * 4;
+    const auto scale = [&](int i) {
+        uint32_t v;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(scales + i * threads * 4) : "memory");
+        if (a.param != QK_F32) {
+            const unsigned odd = (unsigned)(reinterpret_cast<uintptr_t>(a.scales) >> 1) + (unsigned)scale_index(a, row, col + 8 * i);
+            v = odd & 1 ? v >> 16 : v & 0xffffu;
         }
+        return v;
+    };
+    r.s[0] = scale(0);
+    if (!WHOLE && !a.scale32) {
+#pragma unroll
+        for (int i = 1; i < 4; ++i) r.s[i] = scale(i);
     }
 }
 
@@ -226,6 +304,25 @@ template <int FDT> __device__ __forceinline__ float load_bias(const LinearArgs &
     using F = typename ElemOf<FDT>::type;
     if (a.bias == nullptr || f >= a.feats) return 0.0f;
     return (float)static_cast<const F *>(a.bias)[e * a.bias_expert + f * a.bias_stride];
+}
+
+// The activation of N values, chosen outside the loop: one activation's code is fetched, not all of them N times.
+template <int N> __device__ __forceinline__ void activate_all(int act, float *z)
+{
+    if (act == QK_ACT_IDENTITY) return;
+    if (act == QK_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = activate(QK_ACT_RELU, z[i]);
+    } else if (act == QK_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = activate(QK_ACT_SILU, z[i]);
+    } else if (act == QK_ACT_GELU_TANH) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = activate(QK_ACT_GELU_TANH, z[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = activate(QK_ACT_GELU, z[i]);
+    }
 }
 
 // One output element from its sum.

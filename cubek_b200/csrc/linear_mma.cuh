@@ -14,6 +14,7 @@
 #pragma once
 
 #include <atomic>
+#include <type_traits>
 
 #include "linear_kernels.cuh"
 #include "sm100.cuh"
@@ -30,8 +31,9 @@ struct LinearMmaArgs {
     int kblocks;      // steps of 64 of the contraction
 };
 
-constexpr int MMA_THREADS = 448;   // warps 0-3 epilogue, 4 loads x, 5 products, 6-13 weight
-constexpr int MMA_WEIGHT_WARPS = 8;
+constexpr int MMA_GROUPS = 2;          // groups of 8 warps that take the weight's steps in turn
+constexpr int MMA_WEIGHT_THREADS = 256;
+constexpr int MMA_THREADS = 192 + MMA_GROUPS * MMA_WEIGHT_THREADS;   // warps 0-3 epilogue, 4 loads x, 5 products, then weight
 constexpr int MMA_MAX_STAGES = 8;
 constexpr int A_BYTES = 128 * 64 * 2;
 constexpr int MMA_SMEM_LIMIT = 226 * 1024;   // dynamic; the barriers are static
@@ -71,35 +73,59 @@ __device__ __forceinline__ MmaTile mma_tile(const LinearMmaArgs &m, const MmaSch
     return r;
 }
 
-// 16 sums of one feature per lane, rows r .. r + 15 of the tile (valid: how many exist).
+// 16 sums of one feature per lane, rows row .. row + 15 of which `valid` exist.
 template <int FDT>
-__device__ __forceinline__ void mma_store16(const LinearArgs &a, const float *v, int row, int valid, int f, float bias, float bias_even, float bias_odd)
+__device__ __forceinline__ void mma_store16(const LinearArgs &a, float *v, int row, int valid, int f, float bias, float bias_even, float bias_odd)
 {
     using F = typename ElemOf<FDT>::type;
     if (a.pairs) {
         // lanes 2i and 2i + 1 hold neighbouring features: the even one takes both of even rows, the odd one of odd rows
-        const int odd = threadIdx.x & 1, fe = f - odd;
+        const int odd = threadIdx.x & 1;
 #pragma unroll
         for (int j = 0; j < 16; j += 2) {
-            const float give = odd ? v[j] : v[j + 1];
-            const float got = __shfl_xor_sync(0xffffffffu, give, 1);
-            float z0 = (odd ? got : v[j]) + bias_even, z1 = (odd ? v[j + 1] : got) + bias_odd;
-            if (j + odd >= valid || f >= a.feats) continue;
-            const long long r = row + j + odd;
-            if (a.pre) *reinterpret_cast<uint32_t *>(static_cast<F *>(a.pre) + r * a.pre_stride + fe) = h2_pack<FDT>(z0, z1);
-            z0 = activate(a.act, z0);
-            z1 = activate(a.act, z1);
-            if (a.residual) {
-                const uint32_t q = *reinterpret_cast<const uint32_t *>(static_cast<const F *>(a.residual) + r * a.residual_stride + fe);
-                z0 += widen_lo<FDT>(q);
-                z1 += widen_hi<FDT>(q);
-            }
-            *reinterpret_cast<uint32_t *>(static_cast<F *>(a.out) + r * a.out_stride + fe) = h2_pack<FDT>(z0, z1);
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+            v[j] = (odd ? got : v[j]) + bias_even;
+            v[j + 1] = (odd ? v[j + 1] : got) + bias_odd;
         }
-    } else {
+        if (f >= a.feats) return;
+        const long long r0 = row + odd;
+        const int fe = f - odd;
+        if (a.pre) {
+            F *p = static_cast<F *>(a.pre) + r0 * a.pre_stride + fe;
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (j < valid && f < a.feats) finish_one<FDT>(a, row + j, f, v[j], bias);
+            for (int j = 0; j < 16; j += 2)
+                if (j + odd < valid) *reinterpret_cast<uint32_t *>(p + j * a.pre_stride) = h2_pack<FDT>(v[j], v[j + 1]);
+        }
+        activate_all<16>(a.act, v);
+        if (a.residual) {
+            const F *p = static_cast<const F *>(a.residual) + r0 * a.residual_stride + fe;
+            uint32_t q[8];
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) q[j / 2] = j + odd < valid ? *reinterpret_cast<const uint32_t *>(p + j * a.residual_stride) : 0u;
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                v[j] += widen_lo<FDT>(q[j / 2]);
+                v[j + 1] += widen_hi<FDT>(q[j / 2]);
+            }
+        }
+        F *p = static_cast<F *>(a.out) + r0 * a.out_stride + fe;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2)
+            if (j + odd < valid) *reinterpret_cast<uint32_t *>(p + j * a.out_stride) = h2_pack<FDT>(v[j], v[j + 1]);
+    } else {
+        if (f >= a.feats) return;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            v[j] += bias;
+            if (a.pre && j < valid) static_cast<F *>(a.pre)[(row + j) * a.pre_stride + f] = (F)v[j];
+        }
+        activate_all<16>(a.act, v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            if (j >= valid) break;
+            if (a.residual) v[j] += (float)static_cast<const F *>(a.residual)[(row + j) * a.residual_stride + f];
+            static_cast<F *>(a.out)[(row + j) * a.out_stride + f] = (F)v[j];
+        }
     }
 }
 
@@ -107,9 +133,8 @@ __device__ __forceinline__ void mma_store16(const LinearArgs &a, const float *v,
 template <int KIND, int FDT, bool BWD, int CG>
 __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid_constant__ CUtensorMap xmap, const LinearMmaArgs m)
 {
-    constexpr int AHEAD = CodeRun<KIND>::WORDS >= 8 ? 3 : 4;   // steps whose codes are in flight to registers
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[3 * MMA_MAX_STAGES + 5];
+    __shared__ __align__(8) uint64_t bars[2 * MMA_MAX_STAGES + 5];
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up;
     const LinearArgs &a = m.a;
@@ -117,22 +142,21 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int b_rows = m.tile_rows / CG;                        // rows of x this CTA loads
     const uint32_t b_bytes = (uint32_t)b_rows * 128u, stage_bytes = A_BYTES + b_bytes;
-    int *table = reinterpret_cast<int *>(smem_raw + (base - smem_u32(smem_raw)) + m.stages * stage_bytes);
+    const uint32_t runs = base + m.stages * stage_bytes, slot_bytes = StagedRuns<KIND>::slot_bytes(MMA_WEIGHT_THREADS, a.scale32);
+    int *table = reinterpret_cast<int *>(smem_raw + (runs - smem_u32(smem_raw)) + MMA_GROUPS * StagedRuns<KIND>::AHEAD * slot_bytes);
     const uint32_t bar0 = smem_u32(bars);
-    const auto full_x = [&](int s) { return bar0 + 8u * s; };
-    const auto full_w = [&](int s) { return bar0 + 8u * (MMA_MAX_STAGES + s); };
-    const auto empty = [&](int s) { return bar0 + 8u * (2 * MMA_MAX_STAGES + s); };
-    const auto acc_full = [&](int b) { return bar0 + 8u * (3 * MMA_MAX_STAGES + b); };
-    const auto acc_empty = [&](int b) { return bar0 + 8u * (3 * MMA_MAX_STAGES + 2 + b); };
-    const uint32_t drained = bar0 + 8u * (3 * MMA_MAX_STAGES + 4);
+    const auto full = [&](int s) { return bar0 + 8u * s; };
+    const auto empty = [&](int s) { return bar0 + 8u * (MMA_MAX_STAGES + s); };
+    const auto acc_full = [&](int b) { return bar0 + 8u * (2 * MMA_MAX_STAGES + b); };
+    const auto acc_empty = [&](int b) { return bar0 + 8u * (2 * MMA_MAX_STAGES + 2 + b); };
+    const uint32_t drained = bar0 + 8u * (2 * MMA_MAX_STAGES + 4);
     const uint32_t rank = (CG == 2 || m.split > 1) ? cluster_rank() : 0u;
     const bool leader = CG == 1 || rank == 0;
 
     if (threadIdx.x == 0) {
         gave_up = 0;
         for (int s = 0; s < MMA_MAX_STAGES; ++s) {
-            mbar_init(full_x(s), 1);
-            mbar_init(full_w(s), MMA_WEIGHT_WARPS * CG);
+            mbar_init(full(s), 1 + 8 * CG);   // the tile of x (with its bytes) and the warps of the weight
             mbar_init(empty(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -202,10 +226,12 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
     const int kb0 = CG == 1 ? (int)((long long)m.kblocks * rank / m.split) : 0;
     const int kb1 = CG == 1 ? (int)((long long)m.kblocks * (rank + 1) / m.split) : m.kblocks;
     constexpr int TILE_FEATS = 128 * CG;
+    const int stages = m.stages;
     int stage = 0, phase = 0;
-    const auto next_stage = [&] {
-        if (++stage == m.stages) {
-            stage = 0;
+    const auto next_stage = [&](int by = 1) {
+        stage += by;
+        if (stage >= stages) {
+            stage -= stages;
             phase ^= 1;
         }
     };
@@ -228,11 +254,11 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
                     if (dead) break;
                     const uint32_t dst = base + stage * stage_bytes + A_BYTES;
                     if (CG == 1) {
-                        mbar_expect_tx(full_x(stage), b_bytes);
-                        tma_load_2d(dst, &xmap, kb * 64, tile.r0, full_x(stage));
+                        mbar_expect_tx(full(stage), b_bytes);
+                        tma_load_2d(dst, &xmap, kb * 64, tile.r0, full(stage));
                     } else {
-                        if (leader) mbar_expect_tx(full_x(stage), 2 * b_bytes);
-                        tma_load_2d_pair(dst, &xmap, kb * 64, tile.r0 + (int)rank * b_rows, full_x(stage));
+                        if (leader) mbar_expect_tx(full(stage), 2 * b_bytes);
+                        tma_load_2d_pair(dst, &xmap, kb * 64, tile.r0 + (int)rank * b_rows, full(stage));
                     }
                     ++started;
                     next_stage();
@@ -248,7 +274,7 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
             for (int i = min(started, m.stages); i > 0; --i) {
                 stage = stage == 0 ? m.stages - 1 : stage - 1;
                 if (stage == m.stages - 1) phase ^= 1;
-                mbar_wait(full_x(stage), phase, nullptr);
+                mbar_wait(full(stage), phase, nullptr);
             }
         }
     } else if (warp == 5) {
@@ -256,26 +282,29 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
         const uint32_t idesc = instr_desc(FDT == QK_BF16, BWD, 128 * CG, m.tile_rows);
         int buf = 0, buf_phase = 0;
         for (int t = first; t < sched.total; t += step) {
-            if (lane == 0 && leader && kb0 < kb1) {
+            if (leader && kb0 < kb1) {
                 wait(acc_empty(buf), buf_phase ^ 1);
                 tc_fence_after();
+                const uint32_t d = tmem + buf * m.tile_rows;
+#pragma unroll 1
                 for (int kb = kb0; kb < kb1; ++kb) {
-                    wait(full_x(stage), phase);
-                    wait(full_w(stage), phase);
+                    wait(full(stage), phase);
+                    dead = __any_sync(0xffffffffu, dead);
                     if (dead) break;
                     tc_fence_after();
-                    const uint32_t sa = base + stage * stage_bytes, sb = sa + A_BYTES;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    if (elect_one()) {
+                        const uint32_t sa = base + stage * stage_bytes;
                         // K-major: 16 steps are 32 bytes of a swizzled row.  MN-major: two groups of 8 rows of 128 bytes.
-                        const uint64_t da = BWD ? smem_desc(sa + i * 2048, 8192, 1024) : smem_desc(sa + i * 32, 16, 1024);
-                        const uint64_t db = smem_desc(sb + i * 32, 16, 1024);
-                        mma_f16<CG>(tmem + buf * m.tile_rows, da, db, idesc, kb > kb0 || i > 0);
+                        const uint64_t da = BWD ? smem_desc(sa, 8192, 1024) : smem_desc(sa, 16, 1024), db = smem_desc(sa + A_BYTES, 16, 1024);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            mma_f16<CG>(d, da + i * (BWD ? 2048 / 16 : 32 / 16), db + i * (32 / 16), idesc, kb > kb0 || i > 0);
+                        mma_commit<CG>(empty(stage));
+                        if (kb == kb1 - 1) mma_commit<CG>(acc_full(buf));
                     }
-                    mma_commit<CG>(empty(stage));
+                    __syncwarp();
                     next_stage();
                 }
-                mma_commit<CG>(acc_full(buf));
                 buf ^= 1;
                 if (buf == 0) buf_phase ^= 1;
             }
@@ -285,43 +314,81 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
                 meet_cta();
             }
         }
-        if (lane == 0 && leader) {   // nothing may be in flight to TMEM when it is freed
-            mma_commit<CG>(drained);
+        if (leader) {   // nothing may be in flight to TMEM when it is freed
+            if (elect_one()) mma_commit<CG>(drained);
+            __syncwarp();
             mbar_wait(drained, 0, nullptr);
         }
         __syncwarp();
     } else if (warp >= 6) {
         // ---- weight -------------------------------------------------------------------------------------
+        // Steps are numbered through all tiles of the CTA; group g takes those that are g modulo the number of groups.  (One
+        // group of 8 warps: 1700 cycles a step, the latency of its instructions; they need more warps to hide in.)
         // A thread's 32 codes of a step: 8 neighbouring lanes store to 8 different 16-byte columns of the swizzle.
-        const int id = threadIdx.x - 6 * 32, half = BWD ? id / 128 : 0;
-        const int r = BWD ? (id / 2) % 64 : id / 2, c = (id & 1) * 4;
+        const int group = (threadIdx.x - 192) / MMA_WEIGHT_THREADS, id = (threadIdx.x - 192) % MMA_WEIGHT_THREADS;
+        const int half = BWD ? id / 128 : 0, r = BWD ? (id / 2) % 64 : id / 2, c = (id & 1) * 4;
         const uint32_t mine = BWD ? half * 8192 + r * 128 : r * 128;
-        CodeRun<KIND> run[AHEAD];
-        int lt = first, lkb = kb0;   // the step that is loaded next
-        MmaTile ltile = {};
-        if (lt < sched.total) ltile = mma_tile(m, sched, lt, TILE_FEATS);
-        const auto load_next = [&](CodeRun<KIND> &q) {
-            if (lt >= sched.total) return;
-            const int f = ltile.f0 + (CG == 2 ? (int)rank * 128 : 0);
-            const int row = BWD ? lkb * 64 + r : f + r, col = BWD ? f + half * 64 + (id & 1) * 32 : lkb * 64 + (id & 1) * 32;
-            load_code_run<KIND>(a, q, ltile.e, row, col);
-            if (++lkb >= kb1) {
-                lkb = kb0;
-                lt += step;
-                if (lt < sched.total) ltile = mma_tile(m, sched, lt, TILE_FEATS);
-            }
-        };
-        if (kb0 < kb1) {
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) load_next(run[i]);
-            int t = first, kb = kb0;
-            while (t < sched.total) {
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    if (t >= sched.total) break;
+        const uint32_t slots = runs + group * StagedRuns<KIND>::AHEAD * slot_bytes;
+        const bool whole = a.code_align == 16 && a.k % 32 == 0 && a.scale32;
+        const auto weight = [&](auto simple) {
+            constexpr bool SIMPLE = decltype(simple)::value;
+            constexpr int AHEAD = StagedRuns<KIND>::AHEAD;
+            const int run_col = half * 64 + (id & 1) * 32, steps = kb1 - kb0;
+            // the step whose codes are copied next
+            int it = first, ikb = kb0 + group, ie = 0, jf = 0;
+            CodeRow irow = {};
+            const auto enter = [&] {
+                while (ikb >= kb1) {
+                    ikb -= steps;
+                    it += step;
+                }
+                if (it >= sched.total) return;
+                const MmaTile tile = mma_tile(m, sched, it, TILE_FEATS);
+                ie = tile.e;
+                jf = tile.f0 + (CG == 2 ? (int)rank * 128 : 0);
+                if (!BWD) irow = code_row(a, ie, jf + r);
+            };
+            uint32_t in_slot = 0, out_slot = 0;
+            const auto copy_next = [&] {
+                if (it < sched.total) {
+                    if (BWD) irow = code_row(a, ie, ikb * 64 + r);
+                    const int col = BWD ? jf + run_col : ikb * 64 + run_col;
+                    if (SIMPLE) stage_whole_run<KIND>(a, slots + in_slot, id, MMA_WEIGHT_THREADS, irow, col);
+                    else stage_code_run<KIND>(a, slots + in_slot, id, MMA_WEIGHT_THREADS, irow, col);
+                    in_slot += slot_bytes;
+                    if (in_slot == AHEAD * slot_bytes) in_slot = 0;
+                    ikb += MMA_GROUPS;
+                    if (ikb >= kb1) enter();
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            enter();
+#pragma unroll 1
+            for (int i = 0; i < AHEAD - 1; ++i) copy_next();
+            int kb = kb0 + group;
+            next_stage(group);
+#pragma unroll 1
+            for (int t = first; t < sched.total; t += step) {
+                CodeRow row = {};
+                int of = 0, oe = 0;
+                if (!SIMPLE || a.param != QK_F32) {
+                    const MmaTile tile = mma_tile(m, sched, t, TILE_FEATS);
+                    oe = tile.e;
+                    of = tile.f0 + (CG == 2 ? (int)rank * 128 : 0);
+                    if (!BWD) row = code_row(a, oe, of + r);
+                }
+#pragma unroll 1
+                for (; kb < kb1; kb += MMA_GROUPS) {
+                    copy_next();
+                    asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+                    CodeRun<KIND> run;
                     uint32_t o[16];
-                    decode_code_run<KIND, FDT>(a, run[i], o);
-                    load_next(run[i]);
+                    const int col = BWD ? of + run_col : kb * 64 + run_col;
+                    if (BWD && a.param != QK_F32) row = code_row(a, oe, kb * 64 + r);
+                    take_code_run<KIND, SIMPLE>(a, run, slots + out_slot, id, MMA_WEIGHT_THREADS, row, col);
+                    out_slot += slot_bytes;
+                    if (out_slot == AHEAD * slot_bytes) out_slot = 0;
+                    decode_code_run<KIND, FDT, SIMPLE>(a, run, SIMPLE ? 32 : codes_left(a, col), o);
                     wait(empty(stage), phase ^ 1);
                     const uint32_t dst = base + stage * stage_bytes + mine;
 #pragma unroll
@@ -332,21 +399,23 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
                     fence_async_shared();
                     __syncwarp();
                     if (lane == 0 && !dead) {
-                        if (CG == 1) mbar_arrive(full_w(stage));
-                        else mbar_arrive_cluster(full_w(stage), 0);
+                        if (CG == 1) mbar_arrive(full(stage));
+                        else mbar_arrive_cluster(full(stage), 0);
                     }
-                    next_stage();
-                    if (++kb >= kb1) {
-                        kb = kb0;
-                        t += step;
-                        if (m.split > 1) {
-                            meet();
-                            meet();
-                            meet_cta();
-                        }
-                    }
+                    next_stage(MMA_GROUPS);
+                }
+                kb -= steps;
+                if (m.split > 1) {
+                    meet();
+                    meet();
+                    meet_cta();
                 }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        };
+        if (kb0 < kb1) {
+            if (whole) weight(std::true_type{});
+            else weight(std::false_type{});
         } else if (m.split > 1) {
             for (int t = first; t < sched.total; t += step) {
                 meet();
@@ -435,6 +504,17 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
     if (warp == 5) {
         tc_fence_after();
         tmem_free<CG>(tmem, m.tmem_columns);
+    }
+}
+
+// Shared memory of the runs in flight.
+inline int mma_run_bytes(int kind, int scale32)
+{
+    constexpr int threads = MMA_GROUPS * MMA_WEIGHT_THREADS;
+    switch (kind_bits(kind)) {
+    case 8: return StagedRuns<KIND_I8>::AHEAD * StagedRuns<KIND_I8>::slot_bytes(threads, scale32);
+    case 4: return StagedRuns<KIND_PACK4>::AHEAD * StagedRuns<KIND_PACK4>::slot_bytes(threads, scale32);
+    default: return StagedRuns<KIND_PACK2>::AHEAD * StagedRuns<KIND_PACK2>::slot_bytes(threads, scale32);
     }
 }
 

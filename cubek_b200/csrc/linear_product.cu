@@ -57,13 +57,14 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     while (m.split < 8 && tiles * m.split * 2 <= cfg.sm_count && m.kblocks / (m.split * 2) >= 4) m.split *= 2;
     const int stage_bytes = A_BYTES + m.tile_rows * 128;
     const int table = grouped ? (3 * a.experts + 1) * 4 : 0;
-    m.stages = (MMA_SMEM_LIMIT - 1024 - table) / stage_bytes;
+    const int runs = mma_run_bytes(kind, a.scale32);
+    m.stages = (MMA_SMEM_LIMIT - 1024 - table - runs) / stage_bytes;   // 3 at least: 48 KiB each, 48 of runs, 12 of table
     if (m.stages > MMA_MAX_STAGES) m.stages = MMA_MAX_STAGES;
     m.tmem_columns = 32;
     while (m.tmem_columns < 2 * m.tile_rows) m.tmem_columns *= 2;
     const long long clusters = cfg.sm_count / m.split;
     const int grid = (int)(tiles < clusters ? tiles : clusters) * m.split;
-    const size_t smem = 1024 + (size_t)m.stages * stage_bytes + table;
+    const size_t smem = 1024 + (size_t)m.stages * stage_bytes + runs + table;
 
     CUtensorMap map = {};
     if (m.kblocks > 0) {

@@ -22,14 +22,14 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarri
 // Arrival on the barrier at the same place in CTA `rank` of the cluster.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar, uint32_t rank)
 {
-    asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %0, %1;\nmbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n}" ::"r"(bar),
+    asm volatile("{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %0, %1;\nmbarrier.arrive.shared::cluster.b64 _, [r];\n}" ::"r"(bar),
                  "r"(rank)
                  : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity)
 {
     uint32_t ok;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
                  : "=r"(ok)
                  : "r"(bar), "r"(parity)
                  : "memory");
@@ -37,9 +37,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity)
 }
 
 // Waits at most two seconds; `stop`: also ends when another thread of the CTA has given up.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const int *stop)
+static __device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, const int *stop)
 {
-    if (mbar_try_wait(bar, parity)) return true;
     unsigned long long start, now;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
     for (int i = 0;; ++i) {
@@ -49,6 +48,18 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const i
             if (now - start > 2000000000ull || (stop && *(const volatile int *)stop)) return false;
         }
     }
+}
+
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const int *stop)
+{
+    return mbar_try_wait(bar, parity) || mbar_wait_long(bar, parity, stop);
+}
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok));
+    return ok != 0;
 }
 
 // ---- cluster --------------------------------------------------------------------------------------------
