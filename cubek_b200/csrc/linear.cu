@@ -76,7 +76,7 @@ static int fill_weight(LinearArgs &a, const QkTensor *values, const QkTensor *pa
     a.code_align = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
     a.scales = params->ptr;
     a.param = s->param;
-    a.scale32 = 1;
+    a.run_scales = 1;
     a.be = 1;
     a.bn = a.bk = make_fastdiv(1);
     a.scale_row = a.scale_col = a.scale_expert = 0;
@@ -105,7 +105,7 @@ static int fill_weight(LinearArgs &a, const QkTensor *values, const QkTensor *pa
     a.scale_expert = strides[0];
     a.scale_row = strides[1];
     a.scale_col = strides[2];
-    a.scale32 = blk[2] % 32 == 0 || blk[2] >= k;
+    a.run_scales = blk[2] % 32 == 0 || blk[2] >= k ? 1 : blk[2] % 16 == 0 ? 2 : 4;
     return QK_OK;
 }
 

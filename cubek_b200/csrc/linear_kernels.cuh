@@ -23,7 +23,7 @@ struct LinearArgs {
     long long scale_row, scale_col, scale_expert;  // elements
     FastDiv bn, bk;
     unsigned be;                      // experts per scale block
-    int scale32;                      // 32 consecutive codes of a row (at a multiple of 32) share a scale; else 8 do
+    int run_scales;                   // scales of 32 consecutive codes of a row (at a multiple of 32): 1, 2 or 4
     // activations: [rows, contraction], row-major
     const void *x;
     long long x_stride;               // elements
@@ -105,7 +105,7 @@ template <int KIND> struct CodeRun {
     static constexpr int BITS = kind_bits(KIND);
     static constexpr int WORDS = BITS;  // 32 codes of BITS bits
     uint32_t w[WORDS];
-    uint32_t s[4];  // raw scale of each 8 codes (with scale32 only s[0])
+    uint32_t s[4];  // raw scales of equal parts
 };
 
 // A weight row: its codes and its scales.
@@ -144,23 +144,37 @@ template <int FDT> __device__ __forceinline__ float scale_value(const LinearArgs
     return round_to<FDT>(s);
 }
 
+// One stored word times its scale, as packed F x2 in element order.  dequant_word, but for 8-bit codes in bf16: byte b (biased
+// to 0 .. 255) in the middle of the mantissa of 2^15 is 32768 + b, and (32768 + b) s - 32896 s is exact in one
+// multiply-add (32896 = 257 * 128, so with the 8 bits of s neither product needs more than 24), which leaves a single rounding.
+template <int FDT, int KIND> __device__ __forceinline__ void decode_word(uint32_t w, float s, uint32_t *o)
+{
+    if constexpr (FDT == QK_BF16 && (KIND == KIND_PACK8 || KIND == KIND_I8)) {
+        const uint32_t b = w ^ 0x80808080u;
+        const float c = -32896.0f * s;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+            float r0, r1;
+            fma2(__uint_as_float(__byte_perm(b, 0x47000000u, 0x7404 + 16 * i)), __uint_as_float(__byte_perm(b, 0x47000000u, 0x7414 + 16 * i)), s, s,
+                 c, c, r0, r1);
+            o[i / 2] = h2_pack<FDT>(r0, r1);
+        }
+    } else {
+        dequant_word<FDT, KIND>(w, s, h2_pack<FDT>(s, s), o);
+    }
+}
+
 // The run as 16 registers of packed F x2, in element order; codes past `valid` are +0 whatever the scale is.
-// WHOLE: one scale and all 32 codes exist.
-template <int KIND, int FDT, bool WHOLE> __device__ __forceinline__ void decode_code_run(const LinearArgs &a, const CodeRun<KIND> &r, int valid, uint32_t *o)
+// NS: scales of a run (1, 2 or 4).  WHOLE: all 32 codes exist.
+template <int KIND, int FDT, int NS, bool WHOLE>
+__device__ __forceinline__ void decode_code_run(const LinearArgs &a, const CodeRun<KIND> &r, int valid, uint32_t *o)
 {
     constexpr int WORDS = CodeRun<KIND>::WORDS, EPW = kind_elems_per_u32(KIND);
-    float s[4];
-    s[0] = scale_value<FDT>(a, r.s[0]);
-    s[1] = s[2] = s[3] = s[0];
-    if (!WHOLE && !a.scale32) {
+    float s[NS];
 #pragma unroll
-        for (int g = 1; g < 4; ++g) s[g] = scale_value<FDT>(a, r.s[g]);
-    }
+    for (int g = 0; g < NS; ++g) s[g] = scale_value<FDT>(a, r.s[g]);
 #pragma unroll
-    for (int i = 0; i < WORDS; ++i) {   // 16 codes of a word: their blocks are multiples of 16 codes
-        const float sc = s[i * EPW / 8];
-        dequant_word<FDT, KIND>(r.w[i], sc, h2_pack<FDT>(sc, sc), o + i * EPW / 2);
-    }
+    for (int i = 0; i < WORDS; ++i) decode_word<FDT, KIND>(r.w[i], s[i * EPW * NS / 32], o + i * EPW / 2);
     if (!WHOLE && valid < 32) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -170,14 +184,13 @@ template <int KIND, int FDT, bool WHOLE> __device__ __forceinline__ void decode_
     }
 }
 
-// Runs on their way from memory: a thread copies its own ones to its own places in shared memory by asynchronous copies
-// of 16, 8 or 4 bytes, several steps ahead, and nothing but the thread itself waits for them.  (Held in registers instead, the
-// unrolled copies of the loop body for each step in flight cost more instruction fetches than the arithmetic: 1600 cycles
-// a step of 128 x 64 codes, 900 with nothing to do.)
+// Runs on their way from memory where they cannot be fetched as tiles: a thread copies its own ones to its own places in
+// shared memory by asynchronous copies of 16, 8 or 4 bytes, several steps ahead, and nothing but the thread itself waits for
+// them.
 template <int KIND> struct StagedRuns {
     static constexpr int WORDS = CodeRun<KIND>::WORDS;
     static constexpr int AHEAD = WORDS >= 8 ? 3 : 4;
-    __host__ __device__ static int slot_bytes(int threads, int scale32) { return threads * (WORDS * 4 + (scale32 ? 4 : 16)); }
+    __host__ __device__ static constexpr int slot_bytes(int threads) { return threads * (WORDS * 4 + 16); }
 };
 
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void *src, int bytes)
@@ -227,9 +240,8 @@ __device__ __forceinline__ void stage_code_run(const LinearArgs &a, uint32_t slo
         }
     }
     const uint32_t scales = slot + threads * WORDS * 4 + id * 4;
-    const int count = a.scale32 ? 1 : 4;
 #pragma unroll 1
-    for (int i = 0; i < count; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const bool take = 8 * i < valid;
         const long long at = take ? scale_index(a, row, col + 8 * i) : 0;
         const uintptr_t q = reinterpret_cast<uintptr_t>(a.scales) + (a.param == QK_F32 ? at * 4 : at * 2);
@@ -237,27 +249,8 @@ __device__ __forceinline__ void stage_code_run(const LinearArgs &a, uint32_t slo
     }
 }
 
-// The same where every run is complete or lies wholly past the weight, starts on 16 bytes (8 for 2-bit codes) and has one scale.
-template <int KIND>
-__device__ __forceinline__ void stage_whole_run(const LinearArgs &a, uint32_t slot, int id, int threads, const CodeRow &row, int col)
-{
-    constexpr int BITS = CodeRun<KIND>::BITS, WORDS = CodeRun<KIND>::WORDS;
-    const bool ok = row.exists && col < a.k;
-    const uint8_t *p = ok ? row.codes + (col * BITS) / 8 : a.codes;
-    if constexpr (WORDS == 2) {
-        copy_async8(slot + id * 8, p, ok ? 8 : 0);
-    } else {
-#pragma unroll
-        for (int i = 0; i < WORDS / 4; ++i) copy_async16(slot + (i * threads + id) * 16, p + 16 * i, ok ? 16 : 0);
-    }
-    const long long at = ok ? scale_index(a, row, col) : 0;
-    const uintptr_t q = reinterpret_cast<uintptr_t>(a.scales) + (a.param == QK_F32 ? at * 4 : at * 2);
-    copy_async4(slot + threads * WORDS * 4 + id * 4, reinterpret_cast<const void *>(q & ~(uintptr_t)3), ok ? 4 : 0);
-}
-
-// The staged run, once its copies have arrived.
-template <int KIND, bool WHOLE>
-__device__ __forceinline__ void take_code_run(const LinearArgs &a, CodeRun<KIND> &r, uint32_t slot, int id, int threads, const CodeRow &row, int col)
+// The codes of a staged run, once its copies have arrived.
+template <int KIND> __device__ __forceinline__ void take_codes(CodeRun<KIND> &r, uint32_t slot, int id, int threads)
 {
     constexpr int WORDS = CodeRun<KIND>::WORDS;
     if constexpr (WORDS == 2) {
@@ -270,21 +263,13 @@ __device__ __forceinline__ void take_code_run(const LinearArgs &a, CodeRun<KIND>
                          : "r"(slot + (i / 4 * threads + id) * 16)
                          : "memory");
     }
-    const uint32_t scales = slot + threads * WORDS * 4 + id * 4;
-    const auto scale = [&](int i) {
-        uint32_t v;
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(scales + i * threads * 4) : "memory");
-        if (a.param != QK_F32) {
-            const unsigned odd = (unsigned)(reinterpret_cast<uintptr_t>(a.scales) >> 1) + (unsigned)scale_index(a, row, col + 8 * i);
-            v = odd & 1 ? v >> 16 : v & 0xffffu;
-        }
-        return v;
-    };
-    r.s[0] = scale(0);
-    if (!WHOLE && !a.scale32) {
-#pragma unroll
-        for (int i = 1; i < 4; ++i) r.s[i] = scale(i);
-    }
+}
+// A scale staged at shared address `from`; `at`: its address in memory (of which the last bits say where in the word it is).
+__device__ __forceinline__ uint32_t take_scale(const LinearArgs &a, uint32_t from, unsigned at)
+{
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+    return a.param == QK_F32 ? v : at & 2 ? v >> 16 : v & 0xffffu;
 }
 
 // ---- epilogue -----------------------------------------------------------------------------------------

@@ -29,14 +29,35 @@ struct LinearMmaArgs {
     int feat_tiles;
     int tmem_columns;
     int kblocks;      // steps of 64 of the contraction
+    // Where aligned rows, whole steps and blocks allow it, codes are fetched as tiles, and a thread's scales lie a constant
+    // number of bytes apart from one of its group's steps to the next.
+    int regular;
+    long long scale_step;
 };
 
 constexpr int MMA_GROUPS = 2;          // groups of 8 warps that take the weight's steps in turn
 constexpr int MMA_WEIGHT_THREADS = 256;
-constexpr int MMA_THREADS = 192 + MMA_GROUPS * MMA_WEIGHT_THREADS;   // warps 0-3 epilogue, 4 loads x, 5 products, then weight
+constexpr int MMA_WEIGHT_FIRST = 224;  // warps 0-3 epilogue, 4 loads x, 5 products, 6 loads codes, then weight
+constexpr int MMA_THREADS = MMA_WEIGHT_FIRST + MMA_GROUPS * MMA_WEIGHT_THREADS;
 constexpr int MMA_MAX_STAGES = 8;
+// Tiles of codes on their way, each one step (128 x 64 codes).
+template <int KIND> struct CodeTiles {
+    static constexpr int BYTES = 128 * 64 * kind_bits(KIND) / 8;
+    static constexpr int SLOTS = kind_bits(KIND) == 8 ? 6 : 8;
+    static constexpr int SCALES_AHEAD = 4;   // steps of a group whose scales are in flight
+};
+constexpr int MMA_MAX_CODE_TILES = 8;
 constexpr int A_BYTES = 128 * 64 * 2;
 constexpr int MMA_SMEM_LIMIT = 226 * 1024;   // dynamic; the barriers are static
+
+// Shared memory of the codes and scales in flight; `scales` of a run, 0: not regular.
+__host__ __device__ inline int mma_run_bytes(int kind, int scales)
+{
+    const int bits = kind_bits(kind), ahead = bits == 8 ? StagedRuns<KIND_I8>::AHEAD : StagedRuns<KIND_PACK4>::AHEAD;
+    if (scales == 0) return MMA_GROUPS * ahead * MMA_WEIGHT_THREADS * (bits * 4 + 16);
+    return (bits == 8 ? CodeTiles<KIND_I8>::SLOTS : CodeTiles<KIND_PACK4>::SLOTS) * 1024 * bits +
+           MMA_GROUPS * CodeTiles<KIND_I8>::SCALES_AHEAD * MMA_WEIGHT_THREADS * 4 * scales;
+}
 
 struct MmaTile {
     int e, f0, r0, rows;
@@ -131,10 +152,10 @@ __device__ __forceinline__ void mma_store16(const LinearArgs &a, float *v, int r
 
 // CG: 1, or 2 for a pair of CTAs that works on one tile of 256 features with 2-CTA instructions.
 template <int KIND, int FDT, bool BWD, int CG>
-__global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid_constant__ CUtensorMap xmap, const LinearMmaArgs m)
+__global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const LinearMmaArgs m)
 {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * MMA_MAX_STAGES + 5];
+    __shared__ __align__(8) uint64_t bars[2 * MMA_MAX_STAGES + 2 * MMA_MAX_CODE_TILES + 5];
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up;
     const LinearArgs &a = m.a;
@@ -142,14 +163,16 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int b_rows = m.tile_rows / CG;                        // rows of x this CTA loads
     const uint32_t b_bytes = (uint32_t)b_rows * 128u, stage_bytes = A_BYTES + b_bytes;
-    const uint32_t runs = base + m.stages * stage_bytes, slot_bytes = StagedRuns<KIND>::slot_bytes(MMA_WEIGHT_THREADS, a.scale32);
-    int *table = reinterpret_cast<int *>(smem_raw + (runs - smem_u32(smem_raw)) + MMA_GROUPS * StagedRuns<KIND>::AHEAD * slot_bytes);
+    const uint32_t runs = base + m.stages * stage_bytes;
+    int *table = reinterpret_cast<int *>(smem_raw + (runs - smem_u32(smem_raw)) + mma_run_bytes(KIND, m.regular ? a.run_scales : 0));
     const uint32_t bar0 = smem_u32(bars);
     const auto full = [&](int s) { return bar0 + 8u * s; };
     const auto empty = [&](int s) { return bar0 + 8u * (MMA_MAX_STAGES + s); };
     const auto acc_full = [&](int b) { return bar0 + 8u * (2 * MMA_MAX_STAGES + b); };
     const auto acc_empty = [&](int b) { return bar0 + 8u * (2 * MMA_MAX_STAGES + 2 + b); };
     const uint32_t drained = bar0 + 8u * (2 * MMA_MAX_STAGES + 4);
+    const auto codes_full = [&](int s) { return bar0 + 8u * (2 * MMA_MAX_STAGES + 5 + s); };
+    const auto codes_empty = [&](int s) { return bar0 + 8u * (2 * MMA_MAX_STAGES + 5 + MMA_MAX_CODE_TILES + s); };
     const uint32_t rank = (CG == 2 || m.split > 1) ? cluster_rank() : 0u;
     const bool leader = CG == 1 || rank == 0;
 
@@ -158,6 +181,10 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
         for (int s = 0; s < MMA_MAX_STAGES; ++s) {
             mbar_init(full(s), 1 + 8 * CG);   // the tile of x (with its bytes) and the warps of the weight
             mbar_init(empty(s), 1);
+        }
+        for (int s = 0; s < MMA_MAX_CODE_TILES; ++s) {
+            mbar_init(codes_full(s), 1);
+            mbar_init(codes_empty(s), 8);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full(b), 1);
@@ -320,43 +347,190 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
             mbar_wait(drained, 0, nullptr);
         }
         __syncwarp();
-    } else if (warp >= 6) {
+    } else if (warp == 6) {
+        // ---- tiles of codes -------------------------------------------------------------------------------
+        constexpr int SLOTS = CodeTiles<KIND>::SLOTS, BITS = kind_bits(KIND);
+        int slot = 0, slot_phase = 0, started = 0;
+        for (int t = first; t < sched.total; t += step) {
+            const MmaTile tile = mma_tile(m, sched, t, TILE_FEATS);
+            const int f = tile.f0 + (CG == 2 ? (int)rank * 128 : 0);
+            if (lane == 0 && m.regular) {
+#pragma unroll 1
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    wait(codes_empty(slot), slot_phase ^ 1);
+                    if (dead) break;
+                    mbar_expect_tx(codes_full(slot), CodeTiles<KIND>::BYTES);
+                    tma_load_3d(runs + slot * CodeTiles<KIND>::BYTES, &wmap, (BWD ? f : kb * 64) * BITS / 8, BWD ? kb * 64 : f, tile.e, codes_full(slot));
+                    ++started;
+                    if (++slot == SLOTS) {
+                        slot = 0;
+                        slot_phase ^= 1;
+                    }
+                }
+            }
+            if (m.split > 1) {
+                meet();
+                meet();
+                meet_cta();
+            }
+        }
+        if (dead) {
+            for (int i = min(started, SLOTS); i > 0; --i) {
+                slot = slot == 0 ? SLOTS - 1 : slot - 1;
+                if (slot == SLOTS - 1) slot_phase ^= 1;
+                mbar_wait(codes_full(slot), slot_phase, nullptr);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 7) {
         // ---- weight -------------------------------------------------------------------------------------
         // Steps are numbered through all tiles of the CTA; group g takes those that are g modulo the number of groups.  (One
         // group of 8 warps: 1700 cycles a step, the latency of its instructions; they need more warps to hide in.)
         // A thread's 32 codes of a step: 8 neighbouring lanes store to 8 different 16-byte columns of the swizzle.
-        const int group = (threadIdx.x - 192) / MMA_WEIGHT_THREADS, id = (threadIdx.x - 192) % MMA_WEIGHT_THREADS;
+        const int group = (threadIdx.x - MMA_WEIGHT_FIRST) / MMA_WEIGHT_THREADS, id = (threadIdx.x - MMA_WEIGHT_FIRST) % MMA_WEIGHT_THREADS;
         const int half = BWD ? id / 128 : 0, r = BWD ? (id / 2) % 64 : id / 2, c = (id & 1) * 4;
         const uint32_t mine = BWD ? half * 8192 + r * 128 : r * 128;
-        const uint32_t slots = runs + group * StagedRuns<KIND>::AHEAD * slot_bytes;
-        const bool whole = a.code_align == 16 && a.k % 32 == 0 && a.scale32;
-        const auto weight = [&](auto simple) {
-            constexpr bool SIMPLE = decltype(simple)::value;
-            constexpr int AHEAD = StagedRuns<KIND>::AHEAD;
-            const int run_col = half * 64 + (id & 1) * 32, steps = kb1 - kb0;
-            // the step whose codes are copied next
-            int it = first, ikb = kb0 + group, ie = 0, jf = 0;
-            CodeRow irow = {};
-            const auto enter = [&] {
-                while (ikb >= kb1) {
-                    ikb -= steps;
-                    it += step;
-                }
-                if (it >= sched.total) return;
-                const MmaTile tile = mma_tile(m, sched, it, TILE_FEATS);
-                ie = tile.e;
-                jf = tile.f0 + (CG == 2 ? (int)rank * 128 : 0);
-                if (!BWD) irow = code_row(a, ie, jf + r);
+        const uint32_t places = 16u * ((unsigned)c ^ (r & 7));   // of the first chunk; the others: exclusive or with 16 j
+        const int steps = kb1 - kb0, run_col = half * 64 + (id & 1) * 32;
+        const auto features = [&](const MmaTile &tile) { return tile.f0 + (CG == 2 ? (int)rank * 128 : 0); };
+        const auto put = [&](const uint32_t *o) {
+            wait(empty(stage), phase ^ 1);
+            const uint32_t dst = base + stage * stage_bytes + mine + places;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst ^ (uint32_t)(16 * j)), "r"(o[4 * j]), "r"(o[4 * j + 1]),
+                             "r"(o[4 * j + 2]), "r"(o[4 * j + 3])
+                             : "memory");
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0 && !dead) {
+                if (CG == 1) mbar_arrive(full(stage));
+                else mbar_arrive_cluster(full(stage), 0);
+            }
+            next_stage(MMA_GROUPS);
+        };
+        const auto finish_tile = [&] {
+            if (m.split > 1) {
+                meet();
+                meet();
+                meet_cta();
+            }
+        };
+        // the step whose codes are copied next: tile and step of the contraction
+        int it = first, ikb = kb0 + group;
+        const auto wrap = [&] {
+            while (ikb >= kb1) {
+                ikb -= steps;
+                it += step;
+            }
+        };
+        // Tiles of codes come by bulk tensor copies, a run's scales (one or two) by the thread's own asynchronous copies.
+        // (All by the threads' own copies: 16 rows a warp are 16 lines an access, 530 us instead of TODO.)
+        const auto regular = [&](auto ns) {
+            constexpr int NS = decltype(ns)::value, AHEAD = CodeTiles<KIND>::SCALES_AHEAD, SLOTS = CodeTiles<KIND>::SLOTS, BITS = kind_bits(KIND);
+            constexpr uint32_t SCALE_SLOT = NS * MMA_WEIGHT_THREADS * 4;
+            const uint32_t ring = runs + SLOTS * CodeTiles<KIND>::BYTES + group * AHEAD * SCALE_SLOT + id * 4, ring_end = ring + AHEAD * SCALE_SLOT;
+            const int scale_size = a.param == QK_F32 ? 4 : 2;
+            const long long part = (long long)scale_size * a.scale_col;   // from one of a run's scales to the next
+            const bool moving = m.scale_step != 0 || NS > 1;
+            const auto scale_at = [&](const MmaTile &tile, int kb) -> uintptr_t {   // 0: past the weight
+                const int row = BWD ? kb * 64 + r : features(tile) + r, col = BWD ? features(tile) + run_col : kb * 64 + run_col;
+                if (row >= a.n || col >= a.k) return 0;
+                return reinterpret_cast<uintptr_t>(a.scales) + scale_index(a, code_row(a, tile.e, row), col) * scale_size;
             };
-            uint32_t in_slot = 0, out_slot = 0;
+            // where the thread's run of a tile starts: chunks of 16 bytes, swizzled as the tensor map says
+            const uint32_t row_at = BWD ? r * 16 * BITS : r * 8 * BITS;
+            const uint32_t chunk = (BWD ? half * 64 + (id & 1) * 32 : (id & 1) * 32) * BITS / 128;
+            const uint32_t swizzle = BITS != 8 ? 0 : BWD ? r & 7 : (r >> 1) & 3;
+            uint32_t in = ring, out = ring;
+            uintptr_t scale = 0;
+            const auto enter = [&] {
+                wrap();
+                if (it < sched.total) scale = scale_at(mma_tile(m, sched, it, TILE_FEATS), ikb);
+            };
             const auto copy_next = [&] {
                 if (it < sched.total) {
-                    if (BWD) irow = code_row(a, ie, ikb * 64 + r);
-                    const int col = BWD ? jf + run_col : ikb * 64 + run_col;
-                    if (SIMPLE) stage_whole_run<KIND>(a, slots + in_slot, id, MMA_WEIGHT_THREADS, irow, col);
-                    else stage_code_run<KIND>(a, slots + in_slot, id, MMA_WEIGHT_THREADS, irow, col);
+#pragma unroll
+                    for (int i = 0; i < NS; ++i)
+                        copy_async4(in + i * MMA_WEIGHT_THREADS * 4, reinterpret_cast<const void *>(scale ? (scale + i * part) & ~(uintptr_t)3 : reinterpret_cast<uintptr_t>(a.codes) & ~(uintptr_t)3),
+                                    scale ? 4 : 0);
+                    in += SCALE_SLOT;
+                    if (in == ring_end) in = ring;
+                    ikb += MMA_GROUPS;
+                    if (ikb >= kb1) enter();
+                    else if (scale) scale += m.scale_step;
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            if (moving) {
+                enter();
+#pragma unroll 1
+                for (int i = 0; i < AHEAD - 1; ++i) copy_next();
+            }
+            int kb = kb0 + group, slot = group, slot_phase = 0;
+            next_stage(group);
+#pragma unroll 1
+            for (int t = first; t < sched.total; t += step) {
+                uintptr_t at = 0;   // address of the decoded run's scale
+                CodeRun<KIND> run;
+                if (!moving || a.param != QK_F32) {
+                    at = scale_at(mma_tile(m, sched, t, TILE_FEATS), moving ? kb : kb0);
+                    if (!moving) run.s[0] = !at ? 0u : a.param == QK_F32 ? __ldg(reinterpret_cast<const uint32_t *>(at)) : (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(at));
+                }
+#pragma unroll 1
+                for (; kb < kb1; kb += MMA_GROUPS) {
+                    uint32_t o[16];
+                    if (moving) {
+                        copy_next();
+                        asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+#pragma unroll
+                        for (int i = 0; i < NS; ++i) run.s[i] = take_scale(a, out + i * MMA_WEIGHT_THREADS * 4, (unsigned)at + (unsigned)(i * part));
+                        at += (unsigned)m.scale_step;
+                        out += SCALE_SLOT;
+                        if (out == ring_end) out = ring;
+                    }
+                    wait(codes_full(slot), slot_phase);
+                    const uint32_t tile_at = runs + slot * CodeTiles<KIND>::BYTES + row_at;
+                    if constexpr (BITS == 2) {
+                        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(run.w[0]), "=r"(run.w[1]) : "r"(tile_at + run_col / 4) : "memory");
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < BITS / 4; ++i)
+                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                         : "=r"(run.w[4 * i]), "=r"(run.w[4 * i + 1]), "=r"(run.w[4 * i + 2]), "=r"(run.w[4 * i + 3])
+                                         : "r"(tile_at + 16 * ((chunk + i) ^ swizzle))
+                                         : "memory");
+                    }
+                    decode_code_run<KIND, FDT, NS, true>(a, run, 32, o);
+                    __syncwarp();
+                    if (lane == 0 && !dead) mbar_arrive(codes_empty(slot));
+                    slot += MMA_GROUPS;
+                    if (slot >= SLOTS) {
+                        slot -= SLOTS;
+                        slot_phase ^= 1;
+                    }
+                    put(o);
+                }
+                kb -= steps;
+                finish_tile();
+            }
+        };
+        const auto irregular = [&] {
+            constexpr int AHEAD = StagedRuns<KIND>::AHEAD;
+            constexpr uint32_t slot_bytes = StagedRuns<KIND>::slot_bytes(MMA_WEIGHT_THREADS);
+            const uint32_t slots = runs + group * AHEAD * slot_bytes, slots_end = slots + AHEAD * slot_bytes;
+            uint32_t in_slot = slots, out_slot = slots;
+            MmaTile itile = {};
+            const auto enter = [&] {
+                wrap();
+                if (it < sched.total) itile = mma_tile(m, sched, it, TILE_FEATS);
+            };
+            const auto copy_next = [&] {
+                if (it < sched.total) {
+                    const CodeRow row = code_row(a, itile.e, BWD ? ikb * 64 + r : features(itile) + r);
+                    stage_code_run<KIND>(a, in_slot, id, MMA_WEIGHT_THREADS, row, BWD ? features(itile) + run_col : ikb * 64 + run_col);
                     in_slot += slot_bytes;
-                    if (in_slot == AHEAD * slot_bytes) in_slot = 0;
+                    if (in_slot == slots_end) in_slot = slots;
                     ikb += MMA_GROUPS;
                     if (ikb >= kb1) enter();
                 }
@@ -369,59 +543,36 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
             next_stage(group);
 #pragma unroll 1
             for (int t = first; t < sched.total; t += step) {
-                CodeRow row = {};
-                int of = 0, oe = 0;
-                if (!SIMPLE || a.param != QK_F32) {
-                    const MmaTile tile = mma_tile(m, sched, t, TILE_FEATS);
-                    oe = tile.e;
-                    of = tile.f0 + (CG == 2 ? (int)rank * 128 : 0);
-                    if (!BWD) row = code_row(a, oe, of + r);
-                }
+                const MmaTile tile = mma_tile(m, sched, t, TILE_FEATS);
 #pragma unroll 1
                 for (; kb < kb1; kb += MMA_GROUPS) {
                     copy_next();
                     asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
                     CodeRun<KIND> run;
                     uint32_t o[16];
-                    const int col = BWD ? of + run_col : kb * 64 + run_col;
-                    if (BWD && a.param != QK_F32) row = code_row(a, oe, kb * 64 + r);
-                    take_code_run<KIND, SIMPLE>(a, run, slots + out_slot, id, MMA_WEIGHT_THREADS, row, col);
-                    out_slot += slot_bytes;
-                    if (out_slot == AHEAD * slot_bytes) out_slot = 0;
-                    decode_code_run<KIND, FDT, SIMPLE>(a, run, SIMPLE ? 32 : codes_left(a, col), o);
-                    wait(empty(stage), phase ^ 1);
-                    const uint32_t dst = base + stage * stage_bytes + mine;
+                    const int col = BWD ? features(tile) + run_col : kb * 64 + run_col;
+                    const CodeRow row = code_row(a, tile.e, BWD ? kb * 64 + r : features(tile) + r);
+                    take_codes<KIND>(run, out_slot, id, MMA_WEIGHT_THREADS);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + (uint32_t)(((c + j) ^ (r & 7)) * 16)), "r"(o[4 * j]),
-                                     "r"(o[4 * j + 1]), "r"(o[4 * j + 2]), "r"(o[4 * j + 3])
-                                     : "memory");
-                    fence_async_shared();
-                    __syncwarp();
-                    if (lane == 0 && !dead) {
-                        if (CG == 1) mbar_arrive(full(stage));
-                        else mbar_arrive_cluster(full(stage), 0);
-                    }
-                    next_stage(MMA_GROUPS);
+                    for (int i = 0; i < 4; ++i)
+                        run.s[i] = take_scale(a, out_slot + MMA_WEIGHT_THREADS * CodeRun<KIND>::WORDS * 4 + (i * MMA_WEIGHT_THREADS + id) * 4,
+                                              (unsigned)reinterpret_cast<uintptr_t>(a.scales) + 2u * (unsigned)scale_index(a, row, col + 8 * i));
+                    out_slot += slot_bytes;
+                    if (out_slot == slots_end) out_slot = slots;
+                    decode_code_run<KIND, FDT, 4, false>(a, run, codes_left(a, col), o);
+                    put(o);
                 }
                 kb -= steps;
-                if (m.split > 1) {
-                    meet();
-                    meet();
-                    meet_cta();
-                }
+                finish_tile();
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
         };
         if (kb0 < kb1) {
-            if (whole) weight(std::true_type{});
-            else weight(std::false_type{});
-        } else if (m.split > 1) {
-            for (int t = first; t < sched.total; t += step) {
-                meet();
-                meet();
-                meet_cta();
-            }
+            if (!m.regular) irregular();
+            else if (a.run_scales == 1) regular(std::integral_constant<int, 1>{});
+            else regular(std::integral_constant<int, 2>{});
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else {
+            for (int t = first; t < sched.total; t += step) finish_tile();
         }
     } else {
         // ---- epilogue -----------------------------------------------------------------------------------
@@ -507,20 +658,30 @@ __global__ void __launch_bounds__(MMA_THREADS, 1) linear_mma_kernel(const __grid
     }
 }
 
-// Shared memory of the runs in flight.
-inline int mma_run_bytes(int kind, int scale32)
+// Whether the weight's steps are regular, and how far apart its scales.
+inline void mma_steps(LinearMmaArgs &m, bool backward)
 {
-    constexpr int threads = MMA_GROUPS * MMA_WEIGHT_THREADS;
-    switch (kind_bits(kind)) {
-    case 8: return StagedRuns<KIND_I8>::AHEAD * StagedRuns<KIND_I8>::slot_bytes(threads, scale32);
-    case 4: return StagedRuns<KIND_PACK4>::AHEAD * StagedRuns<KIND_PACK4>::slot_bytes(threads, scale32);
-    default: return StagedRuns<KIND_PACK2>::AHEAD * StagedRuns<KIND_PACK2>::slot_bytes(threads, scale32);
-    }
+    const LinearArgs &a = m.a;
+    const long long rows = 64 * MMA_GROUPS, size = a.param == QK_F32 ? 4 : 2;
+    const unsigned block = backward ? a.bn.div : a.bk.div;
+    const long long scale_step = backward ? a.scale_row : a.scale_col;
+    const bool one = scale_step == 0;
+    m.regular = a.code_align == 16 && a.k % 32 == 0 && a.contraction % 64 == 0 && a.run_scales <= 2 && (one || rows % block == 0);
+    m.scale_step = one ? 0 : rows / block * scale_step * size;
+}
+
+// Tile shape of the codes: {bytes, rows} and the swizzle that the kernel undoes.
+inline CUtensorMapSwizzle mma_code_box(bool backward, int bits, cuuint32_t *box)
+{
+    box[0] = (backward ? 128 : 64) * bits / 8;
+    box[1] = backward ? 64 : 128;
+    box[2] = 1;
+    return bits != 8 ? CU_TENSOR_MAP_SWIZZLE_NONE : backward ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
 }
 
 // ---- launch -------------------------------------------------------------------------------------------------
 template <int KIND, int FDT, bool BWD, int CG>
-static cudaError_t launch_mma_one(const CUtensorMap &map, const LinearMmaArgs &m, int grid, size_t smem, const LaunchCfg &cfg, cudaStream_t stream)
+static cudaError_t launch_mma_one(const CUtensorMap &xmap, const CUtensorMap &wmap, const LinearMmaArgs &m, int grid, size_t smem, const LaunchCfg &cfg, cudaStream_t stream)
 {
     static std::atomic<unsigned long long> ready{0};   // devices whose shared-memory limit of this kernel is raised
     int dev = 0;
@@ -550,21 +711,21 @@ static cudaError_t launch_mma_one(const CUtensorMap &map, const LinearMmaArgs &m
     }
     c.attrs = attr;
     c.numAttrs = n;
-    return cudaLaunchKernelEx(&c, linear_mma_kernel<KIND, FDT, BWD, CG>, map, m);
+    return cudaLaunchKernelEx(&c, linear_mma_kernel<KIND, FDT, BWD, CG>, xmap, wmap, m);
 }
 
 template <int FDT, bool BWD, int CG>
-static cudaError_t launch_mma_kind(int kind, const CUtensorMap &map, const LinearMmaArgs &m, int grid, size_t smem, const LaunchCfg &cfg,
+static cudaError_t launch_mma_kind(int kind, const CUtensorMap &xmap, const CUtensorMap &wmap, const LinearMmaArgs &m, int grid, size_t smem, const LaunchCfg &cfg,
                                    cudaStream_t stream)
 {
     switch (kind) {
     case KIND_PACK8:   // bytes either way
-    case KIND_I8: return launch_mma_one<KIND_I8, FDT, BWD, CG>(map, m, grid, smem, cfg, stream);
-    case KIND_PACK4: return launch_mma_one<KIND_PACK4, FDT, BWD, CG>(map, m, grid, smem, cfg, stream);
-    case KIND_PACK2: return launch_mma_one<KIND_PACK2, FDT, BWD, CG>(map, m, grid, smem, cfg, stream);
-    case KIND_E2M1: return launch_mma_one<KIND_E2M1, FDT, BWD, CG>(map, m, grid, smem, cfg, stream);
-    case KIND_E4M3: return launch_mma_one<KIND_E4M3, FDT, BWD, CG>(map, m, grid, smem, cfg, stream);
-    case KIND_E5M2: return launch_mma_one<KIND_E5M2, FDT, BWD, CG>(map, m, grid, smem, cfg, stream);
+    case KIND_I8: return launch_mma_one<KIND_I8, FDT, BWD, CG>(xmap, wmap, m, grid, smem, cfg, stream);
+    case KIND_PACK4: return launch_mma_one<KIND_PACK4, FDT, BWD, CG>(xmap, wmap, m, grid, smem, cfg, stream);
+    case KIND_PACK2: return launch_mma_one<KIND_PACK2, FDT, BWD, CG>(xmap, wmap, m, grid, smem, cfg, stream);
+    case KIND_E2M1: return launch_mma_one<KIND_E2M1, FDT, BWD, CG>(xmap, wmap, m, grid, smem, cfg, stream);
+    case KIND_E4M3: return launch_mma_one<KIND_E4M3, FDT, BWD, CG>(xmap, wmap, m, grid, smem, cfg, stream);
+    case KIND_E5M2: return launch_mma_one<KIND_E5M2, FDT, BWD, CG>(xmap, wmap, m, grid, smem, cfg, stream);
     default: return cudaErrorInvalidValue;
     }
 }

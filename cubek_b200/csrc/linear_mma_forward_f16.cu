@@ -2,9 +2,9 @@
 
 namespace qk {
 
-cudaError_t launch_mma_forward_f16(int kind, const CUtensorMap &map, const LinearMmaArgs &m, int grid, size_t smem, const LaunchCfg &cfg, cudaStream_t stream)
+cudaError_t launch_mma_forward_f16(int kind, const CUtensorMap &xmap, const CUtensorMap &wmap, const LinearMmaArgs &m, int grid, size_t smem, const LaunchCfg &cfg, cudaStream_t stream)
 {
-    return launch_mma_kind<QK_F16, false, 1>(kind, map, m, grid, smem, cfg, stream);
+    return launch_mma_kind<QK_F16, false, 1>(kind, xmap, wmap, m, grid, smem, cfg, stream);
 }
 
 }  // namespace qk

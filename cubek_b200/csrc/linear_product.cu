@@ -5,10 +5,10 @@
 
 namespace qk {
 
-cudaError_t launch_mma_forward_f16(int, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
-cudaError_t launch_mma_forward_bf16(int, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
-cudaError_t launch_mma_backward_f16(int, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
-cudaError_t launch_mma_backward_bf16(int, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
+cudaError_t launch_mma_forward_f16(int, const CUtensorMap &, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
+cudaError_t launch_mma_forward_bf16(int, const CUtensorMap &, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
+cudaError_t launch_mma_backward_f16(int, const CUtensorMap &, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
+cudaError_t launch_mma_backward_bf16(int, const CUtensorMap &, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
 
 bool product_needs_aligned_rows(long long rows, const void *x, long long stride)
 {
@@ -57,7 +57,8 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     while (m.split < 8 && tiles * m.split * 2 <= cfg.sm_count && m.kblocks / (m.split * 2) >= 4) m.split *= 2;
     const int stage_bytes = A_BYTES + m.tile_rows * 128;
     const int table = grouped ? (3 * a.experts + 1) * 4 : 0;
-    const int runs = mma_run_bytes(kind, a.scale32);
+    mma_steps(m, backward);
+    const int runs = mma_run_bytes(kind, m.regular ? a.run_scales : 0);
     m.stages = (MMA_SMEM_LIMIT - 1024 - table - runs) / stage_bytes;   // 3 at least: 48 KiB each, 48 of runs, 12 of table
     if (m.stages > MMA_MAX_STAGES) m.stages = MMA_MAX_STAGES;
     m.tmem_columns = 32;
@@ -66,21 +67,34 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     const int grid = (int)(tiles < clusters ? tiles : clusters) * m.split;
     const size_t smem = 1024 + (size_t)m.stages * stage_bytes + runs + table;
 
-    CUtensorMap map = {};
+    CUtensorMap xmap = {}, wmap = {};
     if (m.kblocks > 0) {
         const EncodeTiled encode = encode_tiled();
         if (!encode) return cudaErrorNotSupported;
+        const cuuint32_t ones[3] = {1, 1, 1};
         const cuuint64_t dims[2] = {(cuuint64_t)a.contraction, (cuuint64_t)a.rows};
         const cuuint64_t strides[1] = {(cuuint64_t)(a.rows > 1 ? a.x_stride * 2 : round_up(a.contraction, 8) * 2ll)};
-        const cuuint32_t box[2] = {64, (cuuint32_t)m.tile_rows}, ones[2] = {1, 1};
-        const CUresult r = encode(&map, fdt == QK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(a.x), dims,
-                                  strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        const cuuint32_t box[2] = {64, (cuuint32_t)m.tile_rows};
+        CUresult r = encode(&xmap, fdt == QK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(a.x), dims, strides,
+                            box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS) return cudaErrorInvalidValue;
+        if (m.regular) {
+            // rows and experts that there is one of may come with any stride: it is not used
+            const long long row_bytes = (long long)a.k * kind_bits(kind) / 8;
+            const cuuint64_t wdims[3] = {(cuuint64_t)row_bytes, (cuuint64_t)a.n, (cuuint64_t)a.experts};
+            const cuuint64_t wstrides[2] = {(cuuint64_t)(a.n > 1 ? a.code_row : (row_bytes + 15) / 16 * 16),
+                                            (cuuint64_t)(a.experts > 1 ? a.code_expert : (row_bytes + 15) / 16 * 16)};
+            cuuint32_t wbox[3];
+            const CUtensorMapSwizzle swizzle = mma_code_box(backward, kind_bits(kind), wbox);
+            r = encode(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(a.codes), wdims, wstrides, wbox, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+            if (r != CUDA_SUCCESS) return cudaErrorInvalidValue;
+        }
     }
     if (fdt == QK_F16)
-        return backward ? launch_mma_backward_f16(kind, map, m, grid, smem, cfg, stream) : launch_mma_forward_f16(kind, map, m, grid, smem, cfg, stream);
-    return backward ? launch_mma_backward_bf16(kind, map, m, grid, smem, cfg, stream) : launch_mma_forward_bf16(kind, map, m, grid, smem, cfg, stream);
+        return backward ? launch_mma_backward_f16(kind, xmap, wmap, m, grid, smem, cfg, stream) : launch_mma_forward_f16(kind, xmap, wmap, m, grid, smem, cfg, stream);
+    return backward ? launch_mma_backward_bf16(kind, xmap, wmap, m, grid, smem, cfg, stream) : launch_mma_forward_bf16(kind, xmap, wmap, m, grid, smem, cfg, stream);
 }
 
 cudaError_t launch_linear_product(int fdt, int kind, bool backward, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
