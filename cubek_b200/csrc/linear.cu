@@ -132,7 +132,8 @@ static int check_offsets(const QkTensor *t, int experts, const void **ptr, int *
 
 static size_t round256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-static bool even_words(const void *p, long long stride) { return reinterpret_cast<uintptr_t>(p) % 4 == 0 && stride % 2 == 0; }
+// Rows of 16-bit elements that start on `bytes`.
+static bool rows_on(int bytes, const void *p, long long stride) { return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride * 2 % bytes == 0; }
 
 // Rows of x that do not start on 16 bytes are copied to ones that do (bulk tensor loads need it).
 static size_t copied_rows_bytes(long long rows, long long cols) { return round256((size_t)rows * ((cols + 7) / 8 * 8) * 2); }
@@ -156,8 +157,12 @@ static int copy_rows(const Matrix &x, int dtype, void *to, long long stride, cud
 
 static int run_product(int dtype, const QkScheme *s, bool backward, LinearArgs &a, cudaStream_t stream)
 {
-    a.pairs = a.feats % 2 == 0 && even_words(a.out, a.out_stride) && (!a.residual || even_words(a.residual, a.residual_stride)) &&
-              (!a.pre || even_words(a.pre, a.pre_stride));
+    const auto all_on = [&](int bytes) {
+        return rows_on(bytes, a.out, a.out_stride) && (!a.residual || rows_on(bytes, a.residual, a.residual_stride)) &&
+               (!a.pre || rows_on(bytes, a.pre, a.pre_stride));
+    };
+    a.pairs = a.feats % 2 == 0 && all_on(4);
+    a.wide = all_on(32);
     a.error_flag = stage_error_flag();
     count_launch();
     return cuda_status(launch_linear_product(dtype, kind_of(s), backward, a, current_cfg(), stream));

@@ -38,7 +38,8 @@ struct LinearArgs {
     void *pre;
     long long pre_stride;
     int act;                          // QkActivation
-    int pairs;                        // two neighbouring features may be read and written as one 32-bit word
+    int pairs;                        // two neighbouring features may be read and written as one 32-bit word,
+    int wide;                         // 16 of them as 32 bytes
     // experts
     const void *offsets;              // nullptr: one expert with all rows
     int offsets64;
@@ -189,7 +190,7 @@ __device__ __forceinline__ void decode_code_run(const LinearArgs &a, const CodeR
 // them.
 template <int KIND> struct StagedRuns {
     static constexpr int WORDS = CodeRun<KIND>::WORDS;
-    static constexpr int AHEAD = WORDS >= 8 ? 3 : 4;
+    static constexpr int AHEAD = WORDS >= 8 ? 2 : 4;
     __host__ __device__ static constexpr int slot_bytes(int threads) { return threads * (WORDS * 4 + 16); }
 };
 

@@ -1,14 +1,21 @@
 // Which kernel a product with a quantized weight takes, and its launch.
 #include "host_checks.cuh"
 #include "linear_backward.cuh"
-#include "linear_mma.cuh"
+#include "linear_narrow.cuh"
+#include "linear_wide.cuh"
 
 namespace qk {
 
-cudaError_t launch_mma_forward_f16(int, const CUtensorMap &, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
-cudaError_t launch_mma_forward_bf16(int, const CUtensorMap &, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
-cudaError_t launch_mma_backward_f16(int, const CUtensorMap &, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
-cudaError_t launch_mma_backward_bf16(int, const CUtensorMap &, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
+#define QK_DECLARE(NAME) cudaError_t NAME(int, const CUtensorMap &, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t)
+QK_DECLARE(launch_narrow_forward_f16);
+QK_DECLARE(launch_narrow_forward_bf16);
+QK_DECLARE(launch_narrow_backward_f16);
+QK_DECLARE(launch_narrow_backward_bf16);
+QK_DECLARE(launch_wide_forward_f16);
+QK_DECLARE(launch_wide_forward_bf16);
+QK_DECLARE(launch_wide_backward_f16);
+QK_DECLARE(launch_wide_backward_bf16);
+#undef QK_DECLARE
 
 bool product_needs_aligned_rows(long long rows, const void *x, long long stride)
 {
@@ -39,32 +46,37 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     LinearMmaArgs m = {};
     m.a = a;
     const bool grouped = a.offsets != nullptr;
+    const int average = a.rows / a.experts;
+    m.kblocks = (a.contraction + 63) / 64;
+    m.feat_tiles = (a.feats + 127) / 128;
+    m.split = 1;
+    const bool wide = average > 256 && m.kblocks > 0;
     long long row_tiles;
-    if (!grouped) {
+    if (wide) {
+        m.tile_rows = WIDE_ROWS;
+    } else if (!grouped) {
         const int tiles = (a.rows + 255) / 256;
         m.tile_rows = round_up((a.rows + tiles - 1) / tiles, 16);
-        row_tiles = tiles;
     } else {
-        const int average = a.rows / a.experts;
         m.tile_rows = average >= 128 ? 256 : round_up(2 * average + 1, 16);
-        row_tiles = a.rows / m.tile_rows + (a.experts < a.rows ? a.experts : a.rows);   // at most
     }
-    m.feat_tiles = (a.feats + 127) / 128;
-    m.kblocks = (a.contraction + 63) / 64;
+    row_tiles = (a.rows + m.tile_rows - 1) / m.tile_rows;
+    if (grouped) row_tiles += a.experts < a.rows ? a.experts : a.rows;   // at most
     const long long tiles = row_tiles * m.feat_tiles;
     if (tiles >= (1ll << 31)) return cudaErrorInvalidConfiguration;
-    m.split = 1;
-    while (m.split < 8 && tiles * m.split * 2 <= cfg.sm_count && m.kblocks / (m.split * 2) >= 4) m.split *= 2;
-    const int stage_bytes = A_BYTES + m.tile_rows * 128;
-    const int table = grouped ? (3 * a.experts + 1) * 4 : 0;
-    mma_steps(m, backward);
-    const int runs = mma_run_bytes(kind, m.regular ? a.run_scales : 0);
-    m.stages = (MMA_SMEM_LIMIT - 1024 - table - runs) / stage_bytes;   // 3 at least: 48 KiB each, 48 of runs, 12 of table
+    if (!wide)
+        while (m.split < 8 && tiles * m.split * 2 <= cfg.sm_count && m.kblocks / (m.split * 2) >= 4) m.split *= 2;
+    mma_steps(m, backward, wide ? WEIGHT_GROUPS : 2);
+    const int stage_bytes = wide ? WIDE_STAGE : A_BYTES + m.tile_rows * 128, table = grouped ? (3 * a.experts + 1) * 4 : 0;
+    const int runs = weight_bytes(kind, m.regular ? a.run_scales : 0, wide ? WIDE_SLOTS : NARROW_SLOTS);
+    // three stages at least (at most 48 KiB each, 64 of runs, 12 of table): the exchange of a split contraction needs 512 bytes a row
+    m.stages = (MMA_SMEM_LIMIT - 1024 - table - runs) / stage_bytes;
     if (m.stages > MMA_MAX_STAGES) m.stages = MMA_MAX_STAGES;
     m.tmem_columns = 32;
     while (m.tmem_columns < 2 * m.tile_rows) m.tmem_columns *= 2;
-    const long long clusters = cfg.sm_count / m.split;
-    const int grid = (int)(tiles < clusters ? tiles : clusters) * m.split;
+    const int members = wide ? 2 : m.split;
+    const long long clusters = cfg.sm_count / members;
+    const int grid = (int)(tiles < clusters ? tiles : clusters) * members;
     const size_t smem = 1024 + (size_t)m.stages * stage_bytes + runs + table;
 
     CUtensorMap xmap = {}, wmap = {};
@@ -74,27 +86,30 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
         const cuuint32_t ones[3] = {1, 1, 1};
         const cuuint64_t dims[2] = {(cuuint64_t)a.contraction, (cuuint64_t)a.rows};
         const cuuint64_t strides[1] = {(cuuint64_t)(a.rows > 1 ? a.x_stride * 2 : round_up(a.contraction, 8) * 2ll)};
-        const cuuint32_t box[2] = {64, (cuuint32_t)m.tile_rows};
+        const cuuint32_t box[2] = {64, (cuuint32_t)(wide ? 128 : m.tile_rows)};
         CUresult r = encode(&xmap, fdt == QK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(a.x), dims, strides,
                             box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS) return cudaErrorInvalidValue;
         if (m.regular) {
-            // rows and experts that there is one of may come with any stride: it is not used
-            const long long row_bytes = (long long)a.k * kind_bits(kind) / 8;
+            // tiles of 64 x 64 codes; rows and experts that there is one of may come with any stride: it is not used
+            const int bits = kind_bits(kind);
+            const long long row_bytes = (long long)a.k * bits / 8;
             const cuuint64_t wdims[3] = {(cuuint64_t)row_bytes, (cuuint64_t)a.n, (cuuint64_t)a.experts};
             const cuuint64_t wstrides[2] = {(cuuint64_t)(a.n > 1 ? a.code_row : (row_bytes + 15) / 16 * 16),
                                             (cuuint64_t)(a.experts > 1 ? a.code_expert : (row_bytes + 15) / 16 * 16)};
-            cuuint32_t wbox[3];
-            const CUtensorMapSwizzle swizzle = mma_code_box(backward, kind_bits(kind), wbox);
+            const cuuint32_t wbox[3] = {(cuuint32_t)(64 * bits / 8), 64, 1};
             r = encode(&wmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(a.codes), wdims, wstrides, wbox, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                       swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                       bits == 8 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
             if (r != CUDA_SUCCESS) return cudaErrorInvalidValue;
         }
     }
-    if (fdt == QK_F16)
-        return backward ? launch_mma_backward_f16(kind, xmap, wmap, m, grid, smem, cfg, stream) : launch_mma_forward_f16(kind, xmap, wmap, m, grid, smem, cfg, stream);
-    return backward ? launch_mma_backward_bf16(kind, xmap, wmap, m, grid, smem, cfg, stream) : launch_mma_forward_bf16(kind, xmap, wmap, m, grid, smem, cfg, stream);
+    using Launch = cudaError_t (*)(int, const CUtensorMap &, const CUtensorMap &, const LinearMmaArgs &, int, size_t, const LaunchCfg &, cudaStream_t);
+    static constexpr Launch launches[2][2][2] = {
+        {{launch_narrow_forward_f16, launch_narrow_forward_bf16}, {launch_narrow_backward_f16, launch_narrow_backward_bf16}},
+        {{launch_wide_forward_f16, launch_wide_forward_bf16}, {launch_wide_backward_f16, launch_wide_backward_bf16}}};
+    return launches[wide][backward][fdt == QK_BF16](kind, xmap, wmap, m, grid, smem, cfg, stream);
 }
 
 cudaError_t launch_linear_product(int fdt, int kind, bool backward, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)

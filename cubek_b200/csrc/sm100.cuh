@@ -148,6 +148,11 @@ template <int CG> __device__ __forceinline__ void mma_commit(uint32_t bar)
                      "h"((unsigned short)3)
                      : "memory");
 }
+// The same for the issuing CTA of a pair alone.
+__device__ __forceinline__ void mma_commit_own(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
 // 16 columns of this warp's 32 lanes.
 __device__ __forceinline__ void tmem_load16(uint32_t addr, float *v)
 {
