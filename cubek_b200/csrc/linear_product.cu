@@ -16,6 +16,8 @@ QK_DECLARE(launch_wide_forward_bf16);
 QK_DECLARE(launch_wide_backward_f16);
 QK_DECLARE(launch_wide_backward_bf16);
 #undef QK_DECLARE
+cudaError_t launch_skinny_f16(int, const LinearArgs &, const LaunchCfg &, cudaStream_t);
+cudaError_t launch_skinny_bf16(int, const LinearArgs &, const LaunchCfg &, cudaStream_t);
 
 bool product_needs_aligned_rows(long long rows, const void *x, long long stride)
 {
@@ -114,6 +116,8 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
 
 cudaError_t launch_linear_product(int fdt, int kind, bool backward, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
 {
+    if (!backward && a.k > 0 && a.rows <= 16 * a.experts)
+        return fdt == QK_F16 ? launch_skinny_f16(kind, a, cfg, stream) : launch_skinny_bf16(kind, a, cfg, stream);
     return launch_mma(fdt, kind, backward, a, cfg, stream);
 }
 
