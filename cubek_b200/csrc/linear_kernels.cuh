@@ -100,6 +100,17 @@ __device__ __forceinline__ float activation_slope(int act, float z)
     }
 }
 
+template <int FDT> __device__ __forceinline__ float widen_lo(uint32_t p)
+{
+    if constexpr (FDT == QK_BF16) return bf16_lo_to_f32(p);
+    else return __low2float(*reinterpret_cast<const __half2 *>(&p));
+}
+template <int FDT> __device__ __forceinline__ float widen_hi(uint32_t p)
+{
+    if constexpr (FDT == QK_BF16) return bf16_hi_to_f32(p);
+    else return __high2float(*reinterpret_cast<const __half2 *>(&p));
+}
+
 // ---- weights ----------------------------------------------------------------------------------------
 // A run of 32 consecutive codes of one weight row, at a column that is a multiple of 32, with its scales as stored.
 template <int KIND> struct CodeRun {
@@ -120,7 +131,8 @@ __device__ __forceinline__ CodeRow code_row(const LinearArgs &a, int e, int row)
 {
     CodeRow c;
     c.codes = a.codes + e * a.code_expert + row * a.code_row;
-    c.scale = (long long)(e / a.be) * a.scale_expert + (long long)fastdiv((unsigned)row, a.bn) * a.scale_row;
+    c.scale = (long long)fastdiv((unsigned)row, a.bn) * a.scale_row;
+    if (e > 0) c.scale += (long long)(a.be == 1 ? e : e / (int)a.be) * a.scale_expert;
     c.exists = row < a.n;
     return c;
 }
@@ -136,20 +148,21 @@ __device__ __forceinline__ long long scale_index(const LinearArgs &a, const Code
     return row.scale + (long long)fastdiv((unsigned)col, a.bk) * a.scale_col;
 }
 
-// RN_F(scale) as f32.
-template <int FDT> __device__ __forceinline__ float scale_value(const LinearArgs &a, uint32_t raw)
+// RN_F(scale) as packed F x2, both halves.
+template <int FDT> __device__ __forceinline__ uint32_t scale_pair(int param, uint32_t raw)
 {
-    const float s = a.param == QK_F32 ? __uint_as_float(raw)
-                    : a.param == QK_BF16 ? __uint_as_float(raw << 16)
-                                         : __half2float(__ushort_as_half((unsigned short)raw));
-    return round_to<FDT>(s);
+    if (param == FDT) return raw * 0x10001u;
+    if (param == QK_F32) return h2_pack<FDT>(__uint_as_float(raw), __uint_as_float(raw));
+    const float s = param == QK_BF16 ? __uint_as_float(raw << 16) : __half2float(__ushort_as_half((unsigned short)raw));
+    return h2_pack<FDT>(s, s);
 }
 
 // One stored word times its scale, as packed F x2 in element order.  dequant_word, but for 8-bit codes in bf16: byte b (biased
 // to 0 .. 255) in the middle of the mantissa of 2^15 is 32768 + b, and (32768 + b) s - 32896 s is exact in one
 // multiply-add (32896 = 257 * 128, so with the 8 bits of s neither product needs more than 24), which leaves a single rounding.
-template <int FDT, int KIND> __device__ __forceinline__ void decode_word(uint32_t w, float s, uint32_t *o)
+template <int FDT, int KIND> __device__ __forceinline__ void decode_word(uint32_t w, uint32_t s2, uint32_t *o)
 {
+    const float s = widen_lo<FDT>(s2);
     if constexpr (FDT == QK_BF16 && (KIND == KIND_PACK8 || KIND == KIND_I8)) {
         const uint32_t b = w ^ 0x80808080u;
         const float c = -32896.0f * s;
@@ -161,7 +174,7 @@ template <int FDT, int KIND> __device__ __forceinline__ void decode_word(uint32_
             o[i / 2] = h2_pack<FDT>(r0, r1);
         }
     } else {
-        dequant_word<FDT, KIND>(w, s, h2_pack<FDT>(s, s), o);
+        dequant_word<FDT, KIND>(w, s, s2, o);
     }
 }
 
@@ -171,9 +184,9 @@ template <int KIND, int FDT, int NS, bool WHOLE>
 __device__ __forceinline__ void decode_code_run(const LinearArgs &a, const CodeRun<KIND> &r, int valid, uint32_t *o)
 {
     constexpr int WORDS = CodeRun<KIND>::WORDS, EPW = kind_elems_per_u32(KIND);
-    float s[NS];
+    uint32_t s[NS];
 #pragma unroll
-    for (int g = 0; g < NS; ++g) s[g] = scale_value<FDT>(a, r.s[g]);
+    for (int g = 0; g < NS; ++g) s[g] = scale_pair<FDT>(a.param, r.s[g]);
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) decode_word<FDT, KIND>(r.w[i], s[i * EPW * NS / 32], o + i * EPW / 2);
     if (!WHOLE && valid < 32) {
@@ -274,17 +287,6 @@ __device__ __forceinline__ uint32_t take_scale(const LinearArgs &a, uint32_t fro
 }
 
 // ---- epilogue -----------------------------------------------------------------------------------------
-template <int FDT> __device__ __forceinline__ float widen_lo(uint32_t p)
-{
-    if constexpr (FDT == QK_BF16) return bf16_lo_to_f32(p);
-    else return __low2float(*reinterpret_cast<const __half2 *>(&p));
-}
-template <int FDT> __device__ __forceinline__ float widen_hi(uint32_t p)
-{
-    if constexpr (FDT == QK_BF16) return bf16_hi_to_f32(p);
-    else return __high2float(*reinterpret_cast<const __half2 *>(&p));
-}
-
 template <int FDT> __device__ __forceinline__ float load_bias(const LinearArgs &a, int e, int f)
 {
     using F = typename ElemOf<FDT>::type;

@@ -51,6 +51,7 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     const int average = a.rows / a.experts;
     m.kblocks = (a.contraction + 63) / 64;
     m.feat_tiles = (a.feats + 127) / 128;
+    m.by_feat_tiles = make_fastdiv((unsigned)m.feat_tiles);
     m.split = 1;
     const bool wide = average > 256 && m.kblocks > 0;
     long long row_tiles;

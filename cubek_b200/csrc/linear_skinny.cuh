@@ -73,8 +73,8 @@ template <bool WHOLE> __device__ __forceinline__ void fetch_x(uint32_t *x, const
     for (int i = 0; i < 2; ++i) {
         if (WHOLE || left <= 8 * i || left >= 8 * i + 8) {
             const uint32_t ok = left > 8 * i;
-            asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %5, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\nmov.b32 %2, 0;\nmov.b32 %3, 0;\n"
-                         "@p ld.global.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
+            asm("{\n.reg .pred p;\nsetp.ne.u32 p, %5, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\nmov.b32 %2, 0;\nmov.b32 %3, 0;\n"
+                "@p ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
                          : "=&r"(x[4 * i]), "=&r"(x[4 * i + 1]), "=&r"(x[4 * i + 2]), "=&r"(x[4 * i + 3])
                          : "l"(p + 8 * i), "r"(ok));
         } else {
@@ -90,27 +90,39 @@ template <bool WHOLE> __device__ __forceinline__ void fetch_x(uint32_t *x, const
 template <int FDT> __device__ __forceinline__ void mma_m16n8k16(float *d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
     if constexpr (FDT == QK_BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 constexpr int SKINNY_FEATS = 16, SKINNY_WARPS = 8;
 
-// 16 of a run's codes (the first or the second half) as packed F x2, in element order; codes past `valid` are +0.
-// NS: scales of a run; 4: any number, and any number of codes.
+// Whether the codes of a word are taken in the order 0, 4, 1, 5, 2, 6, 3, 7, for which x is put in the same order: fields that
+// are 16 bits apart come out of a word with one shift and one logical instruction per pair.
+template <int KIND, int NS> constexpr bool split_pairs = KIND == KIND_PACK4 && NS < 4;
+
+// 16 of a run's codes (the first or the second half) as packed F x2, in element order (or the other); codes past `valid`
+// are +0.  NS: scales of a run; 4: any number, and any number of codes.
 template <int KIND, int FDT, int NS>
 __device__ __forceinline__ void decode_half_run(const LinearArgs &a, const CodeRun<KIND> &r, int half, int valid, uint32_t *o)
 {
     constexpr int WORDS = CodeRun<KIND>::WORDS / 2, EPW = kind_elems_per_u32(KIND);
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) {
-        const float s = scale_value<FDT>(a, r.s[NS == 1 ? 0 : NS == 2 ? half : 2 * half + i * EPW / 8]);
-        decode_word<FDT, KIND>(r.w[half * WORDS + i], s, o + i * EPW / 2);
+        const uint32_t s = scale_pair<FDT>(a.param, r.s[NS == 1 ? 0 : NS == 2 ? half : 2 * half + i * EPW / 8]);
+        const uint32_t w = r.w[half * WORDS + i];
+        if constexpr (split_pairs<KIND, NS>) {
+            constexpr uint32_t BASE = (FDT == QK_BF16) ? 0x43084308u : 0x64086408u;   // 128 or 1024, and the bias of a code
+            const uint32_t bias = h2_const<FDT>(FDT == QK_BF16 ? 136.0f : 1032.0f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[4 * i + j] = h2_mul<FDT>(h2_sub<FDT>((w >> 4 * j & 0x000F000Fu) ^ BASE, bias), s);
+        } else {
+            decode_word<FDT, KIND>(w, s, o + i * EPW / 2);
+        }
     }
     if (NS == 4 && valid < 16 * half + 16) {
 #pragma unroll
@@ -220,6 +232,18 @@ __global__ void __launch_bounds__(32 * SKINNY_WARPS, 2) linear_skinny_kernel(con
 #pragma unroll
                     for (int n = 0; n < NT; ++n)   // rows past the tile repeat its last one; their sums are not stored
                         fetch_x<WHOLE>(x[n], x0[n] + c * 128 + 16 * h, k - col - 16 * h);
+                    if constexpr (split_pairs<KIND, NS>) {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int j = 0; j < 8; j += 4) {
+                                const uint32_t y0 = x[n][j], y1 = x[n][j + 1], y2 = x[n][j + 2], y3 = x[n][j + 3];
+                                x[n][j] = __byte_perm(y0, y2, 0x5410);
+                                x[n][j + 1] = __byte_perm(y0, y2, 0x7632);
+                                x[n][j + 2] = __byte_perm(y1, y3, 0x5410);
+                                x[n][j + 3] = __byte_perm(y1, y3, 0x7632);
+                            }
+                    }
                     decode_half_run<KIND, FDT, NS>(a, q0[i], h, left, o0);
                     decode_half_run<KIND, FDT, NS>(a, q1[i], h, left, o1);
                     if (h == 1) fetch_next(i);
@@ -269,6 +293,7 @@ template <int KIND, int FDT, int NT, int NS> static cudaError_t launch_skinny_ro
     m.a = a;
     m.tile_rows = 8 * NT;
     m.feat_tiles = (a.feats + SKINNY_FEATS - 1) / SKINNY_FEATS;
+    m.by_feat_tiles = make_fastdiv((unsigned)m.feat_tiles);
     const bool grouped = a.offsets != nullptr;
     long long tiles = (a.rows + m.tile_rows - 1) / m.tile_rows;
     if (grouped) tiles += a.experts < a.rows ? a.experts : a.rows;   // at most

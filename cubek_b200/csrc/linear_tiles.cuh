@@ -16,6 +16,7 @@ struct LinearMmaArgs {
     int stages;
     int split;        // CTAs of a cluster that share a tile's contraction
     int feat_tiles;
+    FastDiv by_feat_tiles;
     int tmem_columns;
     int kblocks;      // steps of 64 of the contraction
     // Where aligned rows, whole steps and blocks allow it, codes are fetched as tiles, and a thread's scales lie a constant
@@ -42,7 +43,7 @@ struct MmaSchedule {
 __device__ __forceinline__ MmaTile mma_tile(const LinearMmaArgs &m, const MmaSchedule &s, int t, int feats_per_tile)
 {
     MmaTile r;
-    const int rt = t / m.feat_tiles;
+    const int rt = (int)fastdiv((unsigned)t, m.by_feat_tiles);
     r.f0 = (t - rt * m.feat_tiles) * feats_per_tile;
     if (s.prefix == nullptr) {
         r.e = 0;
