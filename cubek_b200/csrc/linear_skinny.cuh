@@ -2,43 +2,20 @@
 //
 // A warp multiplies 16 features with 8 or 16 rows of x over a slice of K, on mma.sync m16n8k16: the tcgen05 tiles need
 // shared memory, barriers and TMEM, whose latencies a read of a few megabytes does not hide, and the work of the tensor cores
-// is nothing here.  Codes go from memory to registers to the instruction: lane 4 g + t of a warp holds 32 consecutive
-// codes of rows g and g + 8, and 32 consecutive elements of row g of x, at the same place t of a chunk of 128; since the
-// contraction may be summed in any order, eight instructions take them four at a time from every lane as if they were in
-// the instruction's order.  The warps of a CTA share K and add their sums in warp order through shared memory.
+// is nothing here.  Lane 4 g + t of a warp takes 32 consecutive codes of rows g and g + 8, and 32 consecutive elements of row g
+// of x, at the same place t of a chunk of 128; since the contraction may be summed in any order, eight instructions take
+// them four at a time from every lane as if they were in the instruction's order.  Groups of 2, 4 or 8 warps share K and
+// add their sums in warp order through shared memory.
+// Codes are on their way two chunks ahead, by asynchronous copies into the warp's own ring in shared memory: whole rows of a
+// chunk at a time, and no registers, so that 24 warps fit an SM (with a ring in registers 16 did, and the latency of the
+// decoding was what 126 us for 235 MB of 4-bit codes went to).
 #pragma once
 
 #include "linear_tiles.cuh"
 
 namespace qk {
 
-// 16 bytes (8 for 2-bit codes) times N straight to registers, or zero: no branch, so that several loads stay in flight.
-template <int WORDS> __device__ __forceinline__ void load_codes_if(uint32_t *w, const uint8_t *p, uint32_t ok)
-{
-    if constexpr (WORDS == 2) {
-        asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %3, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\n@p ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n}"
-                     : "=&r"(w[0]), "=&r"(w[1])
-                     : "l"(p), "r"(ok));
-    } else {
-#pragma unroll
-        for (int i = 0; i < WORDS; i += 4)
-            asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %5, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\nmov.b32 %2, 0;\nmov.b32 %3, 0;\n"
-                         "@p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
-                         : "=&r"(w[i]), "=&r"(w[i + 1]), "=&r"(w[i + 2]), "=&r"(w[i + 3])
-                         : "l"(p + 4 * i), "r"(ok));
-    }
-}
-__device__ __forceinline__ uint32_t load_scale_if(uintptr_t at, uint32_t wide, uint32_t ok)
-{
-    uint32_t s;
-    asm volatile("{\n.reg .pred w, h, p;\nsetp.ne.u32 p, %3, 0;\nsetp.ne.and.u32 w, %2, 0, p;\nsetp.eq.and.u32 h, %2, 0, p;\nmov.b32 %0, 0;\n"
-                 "@w ld.global.nc.u32 %0, [%1];\n@h ld.global.nc.u16 %0, [%1];\n}"
-                 : "=&r"(s)
-                 : "l"(at), "r"(wide), "r"(ok));
-    return s;
-}
-
-// A run of 32 codes of any size and alignment.
+// A run of 32 codes of any size and alignment, straight to registers.
 template <int KIND> __device__ __forceinline__ void fetch_run(const LinearArgs &a, CodeRun<KIND> &r, const CodeRow &row, int col)
 {
     constexpr int BITS = CodeRun<KIND>::BITS, WORDS = CodeRun<KIND>::WORDS;
@@ -133,195 +110,270 @@ __device__ __forceinline__ void decode_half_run(const LinearArgs &a, const CodeR
     }
 }
 
-// Chunks of a warp are 8 * 128 codes apart.  Regular: aligned rows of whole runs with one or two scales, which then lie a
-// constant distance apart too.
+// Regular: aligned rows of whole runs with one or two scales, which then lie a constant distance, whole words, apart from one
+// of a warp's chunks (at least 2 * 128 codes apart) to the next, an expert's within 2 GiB.
 inline bool skinny_regular(const LinearArgs &a)
 {
-    return a.code_align == 16 && a.k % 32 == 0 && a.run_scales <= 2 && (a.scale_col == 0 || 128 * SKINNY_WARPS % a.bk.div == 0);
+    const double extent = ((a.n - 1) / (double)a.bn.div * a.scale_row + (a.k - 1) / (double)a.bk.div * a.scale_col + 1) * 4;
+    return a.code_align == 16 && a.k % 32 == 0 && a.run_scales <= 2 && (a.scale_col == 0 || 128 % a.bk.div == 0) && extent < 2e9;
 }
 
-// NT: rows of x in eights.  NS: scales of a run, or 4: not regular.  A persistent CTA walks blocks of 16 features (of each
-// group of rows of each expert); codes of the next ones are on their way while one is finished.
-template <int KIND, int FDT, int NT, int NS>
-__global__ void __launch_bounds__(32 * SKINNY_WARPS, 2) linear_skinny_kernel(const LinearMmaArgs m)
+constexpr int SKINNY_SLOTS = 3;
+// Shared memory: a ring per warp, and the warps' sums.
+__host__ __device__ constexpr int skinny_ring_bytes(int bits, int r, int ns) { return SKINNY_SLOTS * r * (256 * bits + 256 * ns); }
+__host__ __device__ constexpr int skinny_bytes(int bits, int nt, int r, int ns)
 {
-    constexpr int BITS = kind_bits(KIND), AHEAD = BITS == 8 ? 2 : 3, ROWS = 8 * NT;
-    constexpr bool WHOLE = NS < 4;
-    __shared__ float part[2][SKINNY_WARPS][ROWS][SKINNY_FEATS];
-    extern __shared__ int table[];
-    const LinearArgs &a = m.a;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
-    pdl_entry();
-    const MmaSchedule sched = mma_schedule(m, table, 32 * SKINNY_WARPS);
-    const int first = blockIdx.x, step = gridDim.x, k = a.k, chunks = (k + 127) / 128;
+    return SKINNY_WARPS * ((ns < 4 ? skinny_ring_bytes(bits, r, ns) : 0) + 8 * nt * SKINNY_FEATS * r * 4);
+}
 
-    // what is fetched next.  Features past the weight read its last row; their sums are not stored.
-    int ft = first, fc = warp;
-    CodeRow row0 = {}, row1 = {};
-    const uint8_t *p0 = nullptr, *p1 = nullptr;
-    uintptr_t s0 = 0, s1 = 0;
+// NT: rows of x in eights.  R: features of a block in sixteens.  NS: scales of a run, or 4: not regular.  A persistent CTA walks
+// blocks of features (of each group of rows of each expert); codes of the next ones are on their way while one is finished.
+// `split`: warps that share a block's K.
+template <int KIND, int FDT, int NT, int R, int NS>
+__global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 && NT == 1 ? 3 : 2) linear_skinny_kernel(const LinearMmaArgs m)
+{
+    constexpr int BITS = kind_bits(KIND), ROWS = 8 * NT, FEATS = SKINNY_FEATS * R, AHEAD = SKINNY_SLOTS - 1;
+    constexpr bool WHOLE = NS < 4;
+    constexpr uint32_t CODES = R * 256 * BITS, SLOT = CODES + R * 256 * NS;   // 16 R rows of 128 codes, and their scales
+    extern __shared__ __align__(128) uint8_t dyn[];
+    const LinearArgs &a = m.a;
+    const int lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
+    const int share = m.split, group = threadIdx.x / 32 / share, warp = threadIdx.x / 32 % share;   // warp of the group
+    float *part = reinterpret_cast<float *>(dyn + (WHOLE ? SKINNY_WARPS * skinny_ring_bytes(BITS, R, NS) : 0)) +
+                  group * share * ROWS * FEATS;   // [warp][row][feature]
+    const auto meet = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * share) : "memory"); };
+    pdl_entry();
+    const MmaSchedule sched = mma_schedule(m, reinterpret_cast<int *>(dyn + skinny_bytes(BITS, NT, R, NS)), 32 * SKINNY_WARPS);
+    const int groups = SKINNY_WARPS / share, first = blockIdx.x * groups + group, step = gridDim.x * groups, k = a.k, chunks = (k + 127) / 128;
     const uint32_t wide = a.param == QK_F32;
     const int scale_size = wide ? 4 : 2;
-    const long long part_step = a.scale_col * scale_size;   // from one of a run's scales to the next
-    const long long scale_step = a.scale_col ? part_step * (128 * SKINNY_WARPS / (int)a.bk.div) : 0;
+    const int part_step = (int)a.scale_col * scale_size;   // bytes from one of a run's scales to the next
+    const int scale_step = a.scale_col ? part_step * (128 * share / (int)a.bk.div) : 0;
+    const auto expert_scales = [&](int e) {
+        return reinterpret_cast<uintptr_t>(a.scales) + (long long)(a.be == 1 ? e : e / (int)a.be) * a.scale_expert * scale_size;
+    };
+    const auto scale_offset = [&](int f) {   // from there, of chunk `warp`
+        return (int)(fastdiv((unsigned)min(f, a.n - 1), a.bn) * a.scale_row + fastdiv((unsigned)(warp * 128 + 32 * t4), a.bk) * a.scale_col) * scale_size;
+    };
+
+    // What is copied next.  A lane copies one piece of 16 bytes of every ROWS_AT_ONCE-th row, so that neighbouring lanes copy
+    // neighbouring pieces.
+    constexpr int PIECES = BITS, ROWS_AT_ONCE = 32 / PIECES, COPIES = 16 * R / ROWS_AT_ONCE;   // 128 codes are BITS pieces
+    const int piece = lane % PIECES, copy_row = lane / PIECES;
+    const uint32_t ring = smem_u32(dyn) + threadIdx.x / 32 * skinny_ring_bytes(BITS, R, NS), ring_end = ring + SKINNY_SLOTS * SLOT;
+    uint32_t in = ring, out = ring;
+    int ft = first, fc = warp;
+    const uint8_t *from = nullptr;
+    const long long row_step = ROWS_AT_ONCE * a.code_row;
+    uintptr_t scales = 0;
+    int scale_from[WHOLE ? 2 * R : 1], rows_left = 0;
     const auto enter = [&] {
         if (ft >= sched.total) return;
-        const MmaTile tile = mma_tile(m, sched, ft, SKINNY_FEATS);
-        row0 = code_row(a, tile.e, min(tile.f0 + g, a.n - 1));
-        row1 = code_row(a, tile.e, min(tile.f0 + g + 8, a.n - 1));
-        if (WHOLE) {
-            const int col = fc * 128 + 32 * t4;
-            p0 = row0.codes + (long long)col * BITS / 8;
-            p1 = row1.codes + (long long)col * BITS / 8;
-            s0 = reinterpret_cast<uintptr_t>(a.scales) + scale_index(a, row0, col) * scale_size;
-            s1 = reinterpret_cast<uintptr_t>(a.scales) + scale_index(a, row1, col) * scale_size;
-        }
-    };
-    CodeRun<KIND> q0[AHEAD], q1[AHEAD];
-    const auto fetch_next = [&](int i) {
-        if (ft >= sched.total || warp >= chunks) return;
-        const int col = fc * 128 + 32 * t4;
-        if constexpr (WHOLE) {
-            const uint32_t ok = col < k;
-            load_codes_if<CodeRun<KIND>::WORDS>(q0[i].w, p0, ok);
-            load_codes_if<CodeRun<KIND>::WORDS>(q1[i].w, p1, ok);
+        const MmaTile tile = mma_tile(m, sched, ft, FEATS);
+        from = a.codes + tile.e * a.code_expert + (tile.f0 + copy_row) * a.code_row + warp * 16 * BITS + piece * 16;
+        rows_left = a.n - tile.f0 - copy_row;
+        scales = expert_scales(tile.e);
 #pragma unroll
-            for (int j = 0; j < NS; ++j) {
-                q0[i].s[j] = load_scale_if(s0 + j * part_step, wide, ok);
-                q1[i].s[j] = load_scale_if(s1 + j * part_step, wide, ok);
+        for (int i = 0; i < 2 * R; ++i) scale_from[i] = scale_offset(tile.f0 + 8 * i + g);
+    };
+    const auto copy_next = [&] {
+        if (ft < sched.total && warp < chunks) {
+            const bool exists = fc * 128 + piece * (128 / PIECES) < k;   // runs of 32 codes exist wholly or not
+#pragma unroll
+            for (int i = 0; i < COPIES; ++i) {
+                const int row = copy_row + i * ROWS_AT_ONCE;
+                const uint32_t at = row * 16 * BITS + 16 * (BITS == 8 ? piece ^ (row & 1) : piece);
+                const bool ok = exists && i * ROWS_AT_ONCE < rows_left;
+                copy_async16(in + at, ok ? from + i * row_step : a.codes, ok ? 16 : 0);
             }
-            p0 += 16 * SKINNY_WARPS * BITS;
-            p1 += 16 * SKINNY_WARPS * BITS;
-            s0 += scale_step;
-            s1 += scale_step;
-        } else {
-            fetch_run<KIND>(a, q0[i], row0, col);
-            fetch_run<KIND>(a, q1[i], row1, col);
+            from += 16 * BITS * share;
+            const int scale_bytes = fc * 128 + 32 * t4 < k ? 4 : 0;
+#pragma unroll
+            for (int i = 0; i < 2 * R; ++i) {
+#pragma unroll
+                for (int j = 0; j < NS; ++j)
+                    copy_async4(in + CODES + ((i * NS + j) * 32 + lane) * 4,
+                                reinterpret_cast<const void *>(scales + (scale_bytes ? scale_from[i] + j * part_step : 0) & ~(uintptr_t)3),
+                                scale_bytes);
+                scale_from[i] += scale_step;
+            }
+            in += SLOT;
+            if (in == ring_end) in = ring;
+            fc += share;
+            if (fc >= chunks) {
+                fc = warp;
+                ft += step;
+                enter();
+            }
         }
-        fc += SKINNY_WARPS;
-        if (fc >= chunks) {
-            fc = warp;
-            ft += step;
-            enter();
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if constexpr (WHOLE) {
+        enter();
+#pragma unroll 1
+        for (int i = 0; i < AHEAD; ++i) copy_next();
+    }
+#pragma unroll 1
+    for (int t = first; t < sched.total; t += step) {
+        const MmaTile tile = mma_tile(m, sched, t, FEATS);
+        const uint16_t *x0[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)   // rows past the tile repeat its last one; their sums are not stored
+            x0[n] = static_cast<const uint16_t *>(a.x) + (long long)(tile.r0 + min(8 * n + g, tile.rows - 1)) * a.x_stride + 32 * t4;
+        uint32_t high = 0;   // which 16-bit scales are the high half of their word
+        if (WHOLE && !wide) {
+#pragma unroll
+            for (int i = 0; i < 2 * R; ++i)
+#pragma unroll
+                for (int j = 0; j < NS; ++j) high |= (uint32_t)(expert_scales(tile.e) + scale_offset(tile.f0 + 8 * i + g) + j * part_step >> 1 & 1) << (i * NS + j);
         }
-    };
-    enter();
+        float acc[R][NT][4] = {};
+#pragma unroll 1
+        for (int c = warp; c < chunks; c += share) {
+            const int col = c * 128 + 32 * t4, left = WHOLE ? 32 : codes_left(a, col);
+            CodeRun<KIND> q[2 * R];
+            if constexpr (WHOLE) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
+                __syncwarp();
+                copy_next();   // into the slot that was read in the step before
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) fetch_next(i);
-
-    int t = first, c = warp, buf = 0;
-    MmaTile tile = {};
-    const uint16_t *x0[NT];
-    const auto start = [&] {
-        if (t >= sched.total) return;
-        tile = mma_tile(m, sched, t, SKINNY_FEATS);
+                for (int i = 0; i < 2 * R; ++i) {
+                    const int row = 8 * i + g;
+                    const uint32_t at = out + row * 16 * BITS;
+                    if constexpr (BITS == 2) {
+                        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(q[i].w[0]), "=r"(q[i].w[1]) : "r"(at + 8 * t4) : "memory");
+                    } else {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) x0[n] = static_cast<const uint16_t *>(a.x) + (long long)(tile.r0 + min(8 * n + g, tile.rows - 1)) * a.x_stride + 32 * t4;
-    };
-    start();
-    float acc[NT][4] = {};
-    while (t < sched.total) {
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            if (t >= sched.total) break;
-            if (c < chunks) {
-                const int col = c * 128 + 32 * t4, left = WHOLE ? 32 : codes_left(a, col);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t x[NT][8], o0[8], o1[8];
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)   // rows past the tile repeat its last one; their sums are not stored
-                        fetch_x<WHOLE>(x[n], x0[n] + c * 128 + 16 * h, k - col - 16 * h);
-                    if constexpr (split_pairs<KIND, NS>) {
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int j = 0; j < 8; j += 4) {
-                                const uint32_t y0 = x[n][j], y1 = x[n][j + 1], y2 = x[n][j + 2], y3 = x[n][j + 3];
-                                x[n][j] = __byte_perm(y0, y2, 0x5410);
-                                x[n][j + 1] = __byte_perm(y0, y2, 0x7632);
-                                x[n][j + 2] = __byte_perm(y1, y3, 0x5410);
-                                x[n][j + 3] = __byte_perm(y1, y3, 0x7632);
-                            }
+                        for (int h = 0; h < BITS / 4; ++h)
+                            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                         : "=r"(q[i].w[4 * h]), "=r"(q[i].w[4 * h + 1]), "=r"(q[i].w[4 * h + 2]), "=r"(q[i].w[4 * h + 3])
+                                         : "r"(at + 16 * (BITS == 8 ? (2 * t4 + h) ^ (row & 1) : t4))
+                                         : "memory");
                     }
-                    decode_half_run<KIND, FDT, NS>(a, q0[i], h, left, o0);
-                    decode_half_run<KIND, FDT, NS>(a, q1[i], h, left, o1);
-                    if (h == 1) fetch_next(i);
+#pragma unroll
+                    for (int j = 0; j < NS; ++j) {
+                        const int s = i * NS + j;
+                        uint32_t v;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(out + CODES + (s * 32 + lane) * 4) : "memory");
+                        q[i].s[j] = wide ? v : high >> s & 1 ? v >> 16 : v & 0xffffu;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2 * R; ++i) {
+                    CodeRow row = code_row(a, tile.e, min(tile.f0 + 8 * i + g, a.n - 1));
+                    row.exists = 1;
+                    fetch_run<KIND>(a, q[i], row, col);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t x[NT][8];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) fetch_x<WHOLE>(x[n], x0[n] + c * 128 + 16 * h, k - col - 16 * h);
+                if constexpr (split_pairs<KIND, NS>) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < 8; j += 4) {
+                            const uint32_t y0 = x[n][j], y1 = x[n][j + 1], y2 = x[n][j + 2], y3 = x[n][j + 3];
+                            x[n][j] = __byte_perm(y0, y2, 0x5410);
+                            x[n][j + 1] = __byte_perm(y0, y2, 0x7632);
+                            x[n][j + 2] = __byte_perm(y1, y3, 0x5410);
+                            x[n][j + 3] = __byte_perm(y1, y3, 0x7632);
+                        }
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    uint32_t o[2][8];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        decode_half_run<KIND, FDT, NS>(a, q[2 * r + i], h, left, o[i]);
+                    }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
-                            mma_m16n8k16<FDT>(acc[n], o0[2 * j], o1[2 * j], o0[2 * j + 1], o1[2 * j + 1], x[n][2 * j], x[n][2 * j + 1]);
+                            mma_m16n8k16<FDT>(acc[r][n], o[0][2 * j], o[1][2 * j], o[0][2 * j + 1], o[1][2 * j + 1], x[n][2 * j], x[n][2 * j + 1]);
                 }
-                c += SKINNY_WARPS;
             }
-            if (c >= chunks) {
-                // the warps' sums of feature g (+ 8) and rows 2 t4, 2 t4 + 1, added in warp order; the two buffers take turns, so
-                // that one barrier is enough
+            out += SLOT;
+            if (out == ring_end) out = ring;
+        }
+        // the warps' sums of features g, g + 8 and rows 2 t4, 2 t4 + 1, added in warp order
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    part[buf][warp][8 * n + 2 * t4][g] = acc[n][0];
-                    part[buf][warp][8 * n + 2 * t4 + 1][g] = acc[n][1];
-                    part[buf][warp][8 * n + 2 * t4][g + 8] = acc[n][2];
-                    part[buf][warp][8 * n + 2 * t4 + 1][g + 8] = acc[n][3];
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[n][j] = 0.0f;
-                }
-                __syncthreads();
-                if ((int)threadIdx.x < ROWS * SKINNY_FEATS) {
-                    const int r = threadIdx.x / SKINNY_FEATS, fi = threadIdx.x % SKINNY_FEATS, f = tile.f0 + fi;
-                    if (r < tile.rows && f < a.feats) {
-                        float s = part[buf][0][r][fi];
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int w = 1; w < SKINNY_WARPS; ++w) s += part[buf][w][r][fi];
-                        finish_one<FDT>(a, tile.r0 + r, f, s, load_bias<FDT>(a, tile.e, f));
-                    }
-                }
-                buf ^= 1;
-                t += step;
-                c = warp;
-                start();
+                for (int j = 0; j < 4; ++j) part[(warp * ROWS + 8 * n + 2 * t4 + (j & 1)) * FEATS + 16 * r + g + (j & 2) * 4] = acc[r][n][j];
+        meet();
+        for (int i = warp * 32 + lane; i < ROWS * FEATS; i += 32 * share) {
+            const int r = i / FEATS, f = tile.f0 + i % FEATS;
+            if (r < tile.rows && f < a.feats) {
+                float sum = part[i];
+                for (int w = 1; w < share; ++w) sum += part[w * ROWS * FEATS + i];
+                finish_one<FDT>(a, tile.r0 + r, f, sum, load_bias<FDT>(a, tile.e, f));
             }
         }
+        meet();
     }
+    if constexpr (WHOLE) asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // ---- launch -------------------------------------------------------------------------------------------------
-template <int KIND, int FDT, int NT, int NS> static cudaError_t launch_skinny_rows(const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
+template <int KIND, int FDT, int NT, int R, int NS> static cudaError_t launch_skinny_rows(const LinearArgs &a, long long row_tiles, const LaunchCfg &cfg, cudaStream_t stream)
 {
+    static std::atomic<unsigned long long> ready{0};
     LinearMmaArgs m = {};
     m.a = a;
     m.tile_rows = 8 * NT;
-    m.feat_tiles = (a.feats + SKINNY_FEATS - 1) / SKINNY_FEATS;
+    m.feat_tiles = (a.feats + SKINNY_FEATS * R - 1) / (SKINNY_FEATS * R);
     m.by_feat_tiles = make_fastdiv((unsigned)m.feat_tiles);
-    const bool grouped = a.offsets != nullptr;
-    long long tiles = (a.rows + m.tile_rows - 1) / m.tile_rows;
-    if (grouped) tiles += a.experts < a.rows ? a.experts : a.rows;   // at most
-    tiles *= m.feat_tiles;
+    const long long tiles = row_tiles * m.feat_tiles, resident = cfg.sm_count * (NS < 4 && NT == 1 ? 3 : 2);
     if (tiles >= (1ll << 31)) return cudaErrorInvalidConfiguration;
-    const int resident = cfg.sm_count * 2;
+    // as few warps to a block as leave four blocks for each group (fewer sums to add, fewer barriers), but no more than chunks
+    m.split = SKINNY_WARPS;
+    while (m.split > 2 && (tiles >= 4 * resident * SKINNY_WARPS * 2 / m.split || m.split > (a.k + 127) / 128)) m.split /= 2;
+    const size_t smem = skinny_bytes(kind_bits(KIND), NT, R, NS) + (a.offsets ? (3 * a.experts + 1) * 4 : 0);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {   // devices whose shared-memory limit of this kernel is raised
+        e = cudaFuncSetAttribute(linear_skinny_kernel<KIND, FDT, NT, R, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
+    }
     cudaLaunchConfig_t c = {};
-    c.gridDim = dim3((unsigned)(tiles < resident ? tiles : resident));
+    const long long ctas = (tiles * m.split + SKINNY_WARPS - 1) / SKINNY_WARPS;
+    c.gridDim = dim3((unsigned)(ctas < resident ? ctas : resident));
     c.blockDim = dim3(32 * SKINNY_WARPS);
-    c.dynamicSmemBytes = grouped ? (3 * a.experts + 1) * 4 : 0;
+    c.dynamicSmemBytes = smem;
     c.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     c.attrs = attr;
     c.numAttrs = cfg.pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&c, linear_skinny_kernel<KIND, FDT, NT, NS>, m);
+    return cudaLaunchKernelEx(&c, linear_skinny_kernel<KIND, FDT, NT, R, NS>, m);
+}
+
+template <int KIND, int FDT, int NT> static cudaError_t launch_skinny_nt(const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
+{
+    long long row_tiles = (a.rows + 8 * NT - 1) / (8 * NT);
+    if (a.offsets) row_tiles += a.experts < a.rows ? a.experts : a.rows;   // at most
+    const int scales = skinny_regular(a) ? a.run_scales : 4;
+    // 32 features a block where that leaves a block for every resident CTA: x is fetched half as often
+    const bool tall = scales < 4 && row_tiles * (a.feats / 32) >= 3ll * cfg.sm_count;
+    if (scales == 4) return launch_skinny_rows<KIND, FDT, NT, 1, 4>(a, row_tiles, cfg, stream);
+    if (scales == 1)
+        return tall ? launch_skinny_rows<KIND, FDT, NT, 2, 1>(a, row_tiles, cfg, stream) : launch_skinny_rows<KIND, FDT, NT, 1, 1>(a, row_tiles, cfg, stream);
+    return tall ? launch_skinny_rows<KIND, FDT, NT, 2, 2>(a, row_tiles, cfg, stream) : launch_skinny_rows<KIND, FDT, NT, 1, 2>(a, row_tiles, cfg, stream);
 }
 
 template <int KIND, int FDT> static cudaError_t launch_skinny_one(const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
 {
-    const int scales = skinny_regular(a) ? a.run_scales : 4;
-    if (a.rows <= 8 * a.experts) {
-        return scales == 1 ? launch_skinny_rows<KIND, FDT, 1, 1>(a, cfg, stream) : scales == 2 ? launch_skinny_rows<KIND, FDT, 1, 2>(a, cfg, stream)
-                                                                                              : launch_skinny_rows<KIND, FDT, 1, 4>(a, cfg, stream);
-    }
-    return scales == 1 ? launch_skinny_rows<KIND, FDT, 2, 1>(a, cfg, stream) : scales == 2 ? launch_skinny_rows<KIND, FDT, 2, 2>(a, cfg, stream)
-                                                                                          : launch_skinny_rows<KIND, FDT, 2, 4>(a, cfg, stream);
+    return a.rows <= 8 * a.experts ? launch_skinny_nt<KIND, FDT, 1>(a, cfg, stream) : launch_skinny_nt<KIND, FDT, 2>(a, cfg, stream);
 }
 
 template <int FDT> static cudaError_t launch_skinny_kind(int kind, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
