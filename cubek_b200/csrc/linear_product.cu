@@ -75,6 +75,7 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     // three stages at least (at most 48 KiB each, 64 of runs, 12 of table): the exchange of a split contraction needs 512 bytes a row
     m.stages = (MMA_SMEM_LIMIT - 1024 - table - runs) / stage_bytes;
     if (m.stages > MMA_MAX_STAGES) m.stages = MMA_MAX_STAGES;
+    if (wide) m.stages = WIDE_STAGES;
     m.tmem_columns = 32;
     while (m.tmem_columns < 2 * m.tile_rows) m.tmem_columns *= 2;
     const int members = wide ? 2 : m.split;

@@ -117,7 +117,7 @@ constexpr int WEIGHT_THREADS = 128, WEIGHT_GROUPS = 4, WEIGHT_SCALES_AHEAD = 4;
 // Shared memory of the codes and scales in flight; `scales` of a run, 0: not regular.
 __host__ __device__ constexpr int weight_bytes(int kind, int scales, int slots)
 {
-    return scales == 0 ? WEIGHT_GROUPS * (kind_bits(kind) == 8 ? StagedRuns<KIND_I8>::AHEAD : StagedRuns<KIND_PACK4>::AHEAD) * WEIGHT_THREADS *
+    return scales == 0 ? WEIGHT_GROUPS * (kind_bits(kind) == 8 ? StagedRuns<KIND_I8>::AHEAD : kind_bits(kind) == 4 ? StagedRuns<KIND_PACK4>::AHEAD : StagedRuns<KIND_PACK2>::AHEAD) * WEIGHT_THREADS *
                              (kind_bits(kind) * 4 + 16)
                        : slots * 512 * kind_bits(kind) + WEIGHT_GROUPS * WEIGHT_SCALES_AHEAD * WEIGHT_THREADS * 4 * scales;
 }
@@ -251,14 +251,17 @@ template <int KIND, int FDT, bool BWD, int STRIDE, int SLOTS> struct WeightWarps
             const uint32_t slots = runs + group * AHEAD * slot_bytes, slots_end = slots + AHEAD * slot_bytes;
             uint32_t in_slot = slots, out_slot = slots;
             MmaTile itile = {};
+            CodeRow irow = {};
             const auto enter = [&] {
                 wrap();
-                if (it < sched.total) itile = mma_tile(m, sched, it, feats_per_tile);
+                if (it >= sched.total) return;
+                itile = mma_tile(m, sched, it, feats_per_tile);
+                if (!BWD) irow = code_row(a, itile.e, features(itile) + r);
             };
             const auto copy_next = [&] {
                 if (it < sched.total) {
-                    const CodeRow row = code_row(a, itile.e, BWD ? ikb * 64 + r : features(itile) + r);
-                    stage_code_run<KIND>(a, in_slot, id, WEIGHT_THREADS, row, BWD ? features(itile) + run_col : ikb * 64 + run_col);
+                    if (BWD) irow = code_row(a, itile.e, ikb * 64 + r);
+                    stage_code_run<KIND>(a, in_slot, id, WEIGHT_THREADS, irow, BWD ? features(itile) + run_col : ikb * 64 + run_col);
                     in_slot += slot_bytes;
                     if (in_slot == slots_end) in_slot = slots;
                     ikb += STRIDE;
@@ -273,6 +276,8 @@ template <int KIND, int FDT, bool BWD, int STRIDE, int SLOTS> struct WeightWarps
 #pragma unroll 1
             for (int t = first; t < sched.total; t += step) {
                 const MmaTile tile = mma_tile(m, sched, t, feats_per_tile);
+                CodeRow row = {};
+                if (!BWD && a.param != QK_F32) row = code_row(a, tile.e, features(tile) + r);
 #pragma unroll 1
                 for (; kb < kb1; kb += STRIDE) {
                     copy_next();
@@ -280,12 +285,16 @@ template <int KIND, int FDT, bool BWD, int STRIDE, int SLOTS> struct WeightWarps
                     CodeRun<KIND> run;
                     uint32_t o[16];
                     const int col = BWD ? features(tile) + run_col : kb * 64 + run_col;
-                    const CodeRow row = code_row(a, tile.e, BWD ? kb * 64 + r : features(tile) + r);
+                    if (BWD && a.param != QK_F32) row = code_row(a, tile.e, kb * 64 + r);
                     take_codes<KIND>(run, out_slot, id, WEIGHT_THREADS);
+                    const uint32_t from = out_slot + WEIGHT_THREADS * CodeRun<KIND>::WORDS * 4 + id * 4;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        run.s[i] = take_scale(a, out_slot + WEIGHT_THREADS * CodeRun<KIND>::WORDS * 4 + (i * WEIGHT_THREADS + id) * 4,
-                                              (unsigned)reinterpret_cast<uintptr_t>(a.scales) + 2u * (unsigned)scale_index(a, row, col + 8 * i));
+                    for (int i = 0; i < 4; ++i) {
+                        const int j = i * a.run_scales / 4, part = 32 / a.run_scales;
+                        unsigned at = 0;
+                        if (a.param != QK_F32) at = (unsigned)reinterpret_cast<uintptr_t>(a.scales) + 2u * (unsigned)scale_index(a, row, col + part * j);
+                        run.s[i] = take_scale(a, from + j * WEIGHT_THREADS * 4, at);
+                    }
                     out_slot += slot_bytes;
                     if (out_slot == slots_end) out_slot = slots;
                     decode_code_run<KIND, FDT, 4, false>(a, run, codes_left(a, col), o);

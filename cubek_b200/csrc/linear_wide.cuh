@@ -17,7 +17,7 @@ constexpr int WIDE_ROWS = 512, WIDE_FEATS = 128;          // tile of a pair
 constexpr int WIDE_FIRST = 224;                           // warps 0-3 epilogue, 4 loads x, 5 products, 6 loads codes, then weight
 constexpr int WIDE_THREADS = WIDE_FIRST + WEIGHT_GROUPS * WEIGHT_THREADS;
 constexpr int WIDE_X_BYTES = 128 * 64 * 2, WIDE_STAGE = 2 * WIDE_X_BYTES + 64 * 64 * 2;
-constexpr int WIDE_SLOTS = 8;
+constexpr int WIDE_SLOTS = 8, WIDE_STAGES = 4;   // 160 KiB, and at most 48 of runs and 12 of table
 
 // 16 sums of neighbouring features f .. f + 15 of one row.
 template <int FDT> __device__ __forceinline__ void wide_store16(const LinearArgs &a, float *v, long long row, int f, const float *bias)
@@ -71,30 +71,29 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) linear_wide_kernel(const __gr
 {
     constexpr int BITS = kind_bits(KIND), TILE_BYTES = 64 * 64 * BITS / 8;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * MMA_MAX_STAGES + 2 * WIDE_SLOTS + 5];
+    __shared__ __align__(8) uint64_t bars[2 * WIDE_STAGES + 2 * WIDE_SLOTS + 5];
     __shared__ float bias_tile[2][WIDE_FEATS];
     __shared__ uint32_t tmem_slot;
     __shared__ int gave_up;
     const LinearArgs &a = m.a;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const int stages = m.stages;
-    const uint32_t runs = base + stages * WIDE_STAGE;
+    const uint32_t runs = base + WIDE_STAGES * WIDE_STAGE;
     int *table = reinterpret_cast<int *>(smem_raw + (runs - smem_u32(smem_raw)) + weight_bytes(KIND, m.regular ? a.run_scales : 0, WIDE_SLOTS));
     const uint32_t bar0 = smem_u32(bars);
     const auto full = [&](int s) { return bar0 + 8u * s; };
-    const auto empty = [&](int s) { return bar0 + 8u * (MMA_MAX_STAGES + s); };
-    const auto acc_full = [&](int b) { return bar0 + 8u * (2 * MMA_MAX_STAGES + b); };
-    const auto acc_empty = [&](int b) { return bar0 + 8u * (2 * MMA_MAX_STAGES + 2 + b); };
-    const uint32_t drained = bar0 + 8u * (2 * MMA_MAX_STAGES + 4);
-    const auto codes_full = [&](int s) { return bar0 + 8u * (2 * MMA_MAX_STAGES + 5 + s); };
-    const auto codes_empty = [&](int s) { return bar0 + 8u * (2 * MMA_MAX_STAGES + 5 + WIDE_SLOTS + s); };
+    const auto empty = [&](int s) { return bar0 + 8u * (WIDE_STAGES + s); };
+    const auto acc_full = [&](int b) { return bar0 + 8u * (2 * WIDE_STAGES + b); };
+    const auto acc_empty = [&](int b) { return bar0 + 8u * (2 * WIDE_STAGES + 2 + b); };
+    const uint32_t drained = bar0 + 8u * (2 * WIDE_STAGES + 4);
+    const auto codes_full = [&](int s) { return bar0 + 8u * (2 * WIDE_STAGES + 5 + s); };
+    const auto codes_empty = [&](int s) { return bar0 + 8u * (2 * WIDE_STAGES + 5 + WIDE_SLOTS + s); };
     const int rank = (int)cluster_rank();
     const bool leader = rank == 0;
 
     if (threadIdx.x == 0) {
         gave_up = 0;
-        for (int s = 0; s < MMA_MAX_STAGES; ++s) {
+        for (int s = 0; s < WIDE_STAGES; ++s) {
             mbar_init(full(s), 1 + 2 * WEIGHT_THREADS / 32);   // the tile of x (with its bytes) and a group's warps of both CTAs
             mbar_init(empty(s), 1);
         }
@@ -129,46 +128,39 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) linear_wide_kernel(const __gr
         }
     };
     const int first = blockIdx.x / 2, step = gridDim.x / 2, steps = m.kblocks;
-    int stage = 0, phase = 0;
-    const auto next_stage = [&](int by) {
-        stage += by;
-        while (stage >= stages) {
-            stage -= stages;
-            phase ^= 1;
-        }
-    };
+    unsigned n = 0;   // steps so far: stage n % 4, and whether it has been used an odd number of times
+    const auto stage = [&] { return (int)(n % WIDE_STAGES); };
+    const auto phase = [&] { return n / WIDE_STAGES & 1; };
 
     if (warp == 4) {
         // ---- rows of x ----------------------------------------------------------------------------------
-        int started = 0;
         for (int t = first; t < sched.total; t += step) {
             const MmaTile tile = mma_tile(m, sched, t, WIDE_FEATS);
             if (lane == 0) {
                 const int parts = tile.rows > 256 ? 2 : 1, row = tile.r0 + rank * 128;
 #pragma unroll 1
                 for (int kb = 0; kb < steps; ++kb) {
-                    wait(empty(stage), phase ^ 1);
+                    wait(empty(stage()), phase() ^ 1);
                     if (dead) break;
-                    const uint32_t dst = base + stage * WIDE_STAGE;
-                    if (leader) mbar_expect_tx(full(stage), 2 * parts * WIDE_X_BYTES);
-                    tma_load_2d_pair(dst, &xmap, kb * 64, row, full(stage));
-                    if (parts > 1) tma_load_2d_pair(dst + WIDE_X_BYTES, &xmap, kb * 64, row + 256, full(stage));
-                    ++started;
-                    next_stage(1);
+                    const uint32_t dst = base + stage() * WIDE_STAGE;
+                    if (leader) mbar_expect_tx(full(stage()), 2 * parts * WIDE_X_BYTES);
+                    tma_load_2d_pair(dst, &xmap, kb * 64, row, full(stage()));
+                    if (parts > 1) tma_load_2d_pair(dst + WIDE_X_BYTES, &xmap, kb * 64, row + 256, full(stage()));
+                    ++n;
                 }
             }
         }
         if (dead && leader) {   // copies in flight still write to this pair's memory: wait for them, again within a limit
-            for (int i = min(started, stages); i > 0; --i) {
-                stage = stage == 0 ? stages - 1 : stage - 1;
-                if (stage == stages - 1) phase ^= 1;
-                mbar_wait(full(stage), phase, nullptr);
+            for (int i = min((int)n, WIDE_STAGES); i > 0; --i) {
+                --n;
+                mbar_wait(full(stage()), phase(), nullptr);
             }
         }
         __syncwarp();
     } else if (warp == 5) {
         // ---- products -----------------------------------------------------------------------------------
         const uint32_t idesc = instr_desc(FDT == QK_BF16, false, 256, WIDE_FEATS) | (BWD ? 1u << 16 : 0u);
+        const uint64_t dx0 = smem_desc(base, 16, 1024), dw0 = smem_desc(base + 2 * WIDE_X_BYTES, BWD ? 8192 : 16, 1024);
         int buf = 0, buf_phase = 0;
         if (leader) {
             for (int t = first; t < sched.total; t += step) {
@@ -177,29 +169,30 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) linear_wide_kernel(const __gr
                 wait(acc_empty(buf), buf_phase ^ 1);
                 tc_fence_after();
                 const uint32_t d = tmem + buf * 256;
+                // A step's eight products take the tensor cores 512 cycles, and this loop has to come round in less.
 #pragma unroll 1
-                for (int kb = 0; kb < steps; ++kb) {
-                    wait(full(stage), phase);
-                    dead = __any_sync(0xffffffffu, dead);
-                    if (dead) break;
+                for (int kb = 0; kb < steps; ++kb, ++n) {
+                    wait(full(stage()), phase());
+                    if (__any_sync(0xffffffffu, dead)) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t sx = base + stage * WIDE_STAGE;
-                        const uint64_t dx = smem_desc(sx, 16, 1024), dw = smem_desc(sx + 2 * WIDE_X_BYTES, BWD ? 8192 : 16, 1024);
+                        const uint32_t at = stage() * (WIDE_STAGE / 16);
+                        const uint64_t dx = dx0 + at, dw = dw0 + at;
+                        mma_f16<2>(d, dx, dw, idesc, kb > 0);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            mma_f16<2>(d, dx + i * (32 / 16), dw + i * (BWD ? 2048 / 16 : 32 / 16), idesc, kb > 0 || i > 0);
+                        for (int i = 1; i < 4; ++i) mma_f16<2>(d, dx + i * (32 / 16), dw + i * (BWD ? 2048 / 16 : 32 / 16), idesc, true);
                         if (second) {
+                            mma_f16<2>(d + 128, dx + WIDE_X_BYTES / 16, dw, idesc, kb > 0);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                mma_f16<2>(d + 128, dx + WIDE_X_BYTES / 16 + i * (32 / 16), dw + i * (BWD ? 2048 / 16 : 32 / 16), idesc, kb > 0 || i > 0);
+                            for (int i = 1; i < 4; ++i)
+                                mma_f16<2>(d + 128, dx + WIDE_X_BYTES / 16 + i * (32 / 16), dw + i * (BWD ? 2048 / 16 : 32 / 16), idesc, true);
                         }
-                        mma_commit<2>(empty(stage));
-                        if (kb == steps - 1) mma_commit<2>(acc_full(buf));
+                        mma_commit<2>(empty(stage()));
                     }
                     __syncwarp();
-                    next_stage(1);
                 }
+                if (elect_one()) mma_commit<2>(acc_full(buf));
+                __syncwarp();
                 buf ^= 1;
                 if (buf == 0) buf_phase ^= 1;
             }
@@ -243,8 +236,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) linear_wide_kernel(const __gr
         const int r = id / 2;
         const uint32_t place = base + 2 * WIDE_X_BYTES + r * 128 + 16u * ((unsigned)((id & 1) * 4) ^ (r & 7));
         const auto put = [&](const uint32_t *o) {
-            wait(empty(stage), phase ^ 1);
-            const uint32_t dst = place + stage * WIDE_STAGE;
+            wait(empty(stage()), phase() ^ 1);
+            const uint32_t dst = place + stage() * WIDE_STAGE;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst ^ (uint32_t)(16 * j)), "r"(o[4 * j]), "r"(o[4 * j + 1]),
@@ -252,10 +245,10 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) linear_wide_kernel(const __gr
                              : "memory");
             fence_async_shared();
             __syncwarp();
-            if (lane == 0 && !dead) mbar_arrive_cluster(full(stage), 0);
-            next_stage(WEIGHT_GROUPS);
+            if (lane == 0 && !dead) mbar_arrive_cluster(full(stage()), 0);
+            n += WEIGHT_GROUPS;
         };
-        next_stage(group);
+        n = group;
         WeightWarps<KIND, FDT, BWD, WEIGHT_GROUPS, WIDE_SLOTS> w{m, sched, first, step, 0, steps, group, group, id, WIDE_FEATS, rank * 64, runs};
         w.run(wait, put, [] {}, codes_full, codes_empty, dead);
     } else {
