@@ -8,6 +8,24 @@
 
 namespace qk {
 
+// g *= act'(z) for N values, chosen outside the loop.
+template <int N> __device__ __forceinline__ void slope_all(int act, float *g, const float *z)
+{
+    if (act == QK_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] *= activation_slope(QK_ACT_RELU, z[i]);
+    } else if (act == QK_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] *= activation_slope(QK_ACT_SILU, z[i]);
+    } else if (act == QK_ACT_GELU_TANH) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] *= activation_slope(QK_ACT_GELU_TANH, z[i]);
+    } else if (act == QK_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) g[i] *= activation_slope(QK_ACT_GELU, z[i]);
+    }
+}
+
 // VEC: elements per access.  8 row lanes of 32 threads; a strip is 32 * VEC columns.
 template <int FDT, int VEC> __global__ void __launch_bounds__(256) activation_backward_kernel(const ActBackwardArgs a)
 {
@@ -28,40 +46,47 @@ template <int FDT, int VEC> __global__ void __launch_bounds__(256) activation_ba
     float sum[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) sum[i] = 0.0f;
+    constexpr int ROWS = VEC == 8 ? 4 : 2;   // rows in flight per thread
     if (col < a.n) {
-        for (int r = (int)min(first, (long long)hi) + ty; r < last; r += 8) {
-            float g[VEC], z[VEC];
-            if constexpr (VEC == 8) {
-                const Vec16 v = ldg128_stream(static_cast<const F *>(a.grad) + r * a.grad_stride + col);
-                widen16<FDT>(v, g);
-                if (a.act != QK_ACT_IDENTITY) {
-                    const Vec16 u = ldg128_stream(static_cast<const F *>(a.pre) + r * a.pre_stride + col);
-                    widen16<FDT>(u, z);
-                }
-            } else {
-                g[0] = (float)static_cast<const F *>(a.grad)[r * a.grad_stride + col];
-                if (a.act != QK_ACT_IDENTITY) z[0] = (float)static_cast<const F *>(a.pre)[r * a.pre_stride + col];
-            }
-            if (a.act != QK_ACT_IDENTITY) {
+        for (long long r0 = first + ty; r0 < last; r0 += 8 * ROWS) {
+            float g[ROWS][VEC], z[ROWS][VEC];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) g[i] *= activation_slope(a.act, z[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) sum[i] += g[i];
-#pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                F *to = static_cast<F *>(d ? a.dz2 : a.dz);
-                if (to == nullptr) continue;
-                to += r * (d ? a.dz2_stride : a.dz_stride) + col;
+            for (int k = 0; k < ROWS; ++k) {
+                const long long r = min(r0 + 8 * k, (long long)last - 1);
                 if constexpr (VEC == 8) {
-                    uint4 v;
-                    v.x = h2_pack<FDT>(g[0], g[1]);
-                    v.y = h2_pack<FDT>(g[2], g[3]);
-                    v.z = h2_pack<FDT>(g[4], g[5]);
-                    v.w = h2_pack<FDT>(g[6], g[7]);
-                    *reinterpret_cast<uint4 *>(to) = v;
+                    const Vec16 v = ldg128_stream(static_cast<const F *>(a.grad) + r * a.grad_stride + col);
+                    widen16<FDT>(v, g[k]);
+                    if (a.act != QK_ACT_IDENTITY) {
+                        const Vec16 u = ldg128_stream(static_cast<const F *>(a.pre) + r * a.pre_stride + col);
+                        widen16<FDT>(u, z[k]);
+                    }
                 } else {
-                    *to = (F)g[0];
+                    g[k][0] = (float)static_cast<const F *>(a.grad)[r * a.grad_stride + col];
+                    if (a.act != QK_ACT_IDENTITY) z[k][0] = (float)static_cast<const F *>(a.pre)[r * a.pre_stride + col];
+                }
+            }
+            slope_all<ROWS * VEC>(a.act, &g[0][0], &z[0][0]);
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k) {
+                const long long r = r0 + 8 * k;
+                if (r >= last) break;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) sum[i] += g[k][i];
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    F *to = static_cast<F *>(d ? a.dz2 : a.dz);
+                    if (to == nullptr) continue;
+                    to += r * (d ? a.dz2_stride : a.dz_stride) + col;
+                    if constexpr (VEC == 8) {
+                        uint4 v;
+                        v.x = h2_pack<FDT>(g[k][0], g[k][1]);
+                        v.y = h2_pack<FDT>(g[k][2], g[k][3]);
+                        v.z = h2_pack<FDT>(g[k][4], g[k][5]);
+                        v.w = h2_pack<FDT>(g[k][6], g[k][7]);
+                        *reinterpret_cast<uint4 *>(to) = v;
+                    } else {
+                        *to = (F)g[k][0];
+                    }
                 }
             }
         }
@@ -92,12 +117,12 @@ template <int FDT> __global__ void __launch_bounds__(256) bias_gradient_kernel(c
     static_cast<F *>(a.grad_bias)[e * a.grad_bias_expert + c * a.grad_bias_stride] = (F)s;
 }
 
-// A few hundred CTAs in all, and no slice below 64 rows of an evenly filled expert.
+// Three CTAs for each of 148 SMs, and no slice below 32 rows of an evenly filled expert.
 int bias_slices(long long rows, long long n, int experts)
 {
     const long long strips = (n + 255) / 256;
-    long long s = 592 / (strips * experts);
-    const long long most = rows / (64ll * experts);
+    long long s = (888 + strips * experts - 1) / (strips * experts);
+    const long long most = rows / (32ll * experts);
     if (s > most) s = most;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }

@@ -323,7 +323,11 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1) linear_narrow_kernel(const 
                 // rows of the tile in shares of `share`; share i is finished by CTA i
                 const int share = m.tile_rows / m.split;
                 meet();
-                for (int r = 0; r < m.tile_rows; r += 16) {
+                int owner = 0, at = 0;
+                const uint32_t mine = base + (rank * share * 128 + threadIdx.x) * 4;
+                uint32_t to = cluster_map(mine, 0);
+#pragma unroll 1
+                for (int r = 0; r < tile.rows; r += 16) {
                     float v[16];
                     if (sums) {
                         tmem_load16(from + r, v);
@@ -333,8 +337,11 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1) linear_narrow_kernel(const 
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int owner = (r + i) / share, at = (r + i) - owner * share;
-                        if (r + i < tile.rows) st_cluster_f32(cluster_map(base + ((rank * share + at) * 128 + threadIdx.x) * 4, owner), v[i]);
+                        if (r + i < tile.rows) st_cluster_f32(to + at * 512, v[i]);
+                        if (++at == share) {
+                            at = 0;
+                            to = cluster_map(mine, min(++owner, m.split - 1));
+                        }
                     }
                 }
                 tc_fence_before();

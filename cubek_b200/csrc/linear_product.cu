@@ -43,6 +43,9 @@ static EncodeTiled encode_tiled()
 
 static int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
+#ifndef WIDE_MIN
+#define WIDE_MIN 256
+#endif
 static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
 {
     LinearMmaArgs m = {};
@@ -53,7 +56,7 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     m.feat_tiles = (a.feats + 127) / 128;
     m.by_feat_tiles = make_fastdiv((unsigned)m.feat_tiles);
     m.split = 1;
-    const bool wide = average > 256 && m.kblocks > 0;
+    const bool wide = average > WIDE_MIN && m.kblocks > 0;
     long long row_tiles;
     if (wide) {
         m.tile_rows = WIDE_ROWS;
@@ -118,7 +121,7 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
 
 cudaError_t launch_linear_product(int fdt, int kind, bool backward, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
 {
-    if (!backward && a.k > 0 && a.rows <= 16 * a.experts)
+    if (!backward && a.k > 0 && a.rows <= 8 * a.experts)
         return fdt == QK_F16 ? launch_skinny_f16(kind, a, cfg, stream) : launch_skinny_bf16(kind, a, cfg, stream);
     return launch_mma(fdt, kind, backward, a, cfg, stream);
 }
