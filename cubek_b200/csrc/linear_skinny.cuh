@@ -1,6 +1,6 @@
 // Products with quantized weights for a handful of rows (single tokens, small decoding batches): bound by reading the codes.
 //
-// A warp multiplies 16 features with 8 or 16 rows of x over a slice of K, on mma.sync m16n8k16: the tcgen05 tiles need
+// A warp multiplies 16 or 32 features with 8 rows of x over a slice of K, on mma.sync m16n8k16: the tcgen05 tiles need
 // shared memory, barriers and TMEM, whose latencies a read of a few megabytes does not hide, and the work of the tensor cores
 // is nothing here.  Lane 4 g + t of a warp takes 32 consecutive codes of rows g and g + 8, and 32 consecutive elements of row g
 // of x, at the same place t of a chunk of 128; since the contraction may be summed in any order, eight instructions take
@@ -76,7 +76,7 @@ template <int FDT> __device__ __forceinline__ void mma_m16n8k16(float *d, uint32
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-constexpr int SKINNY_FEATS = 16, SKINNY_WARPS = 8;
+constexpr int SKINNY_FEATS = 16, SKINNY_ROWS = 8, SKINNY_WARPS = 8;
 
 // Whether the codes of a word are taken in the order 0, 4, 1, 5, 2, 6, 3, 7, for which x is put in the same order: fields that
 // are 16 bits apart come out of a word with one shift and one logical instruction per pair.
@@ -121,18 +121,18 @@ inline bool skinny_regular(const LinearArgs &a)
 constexpr int SKINNY_SLOTS = 3;
 // Shared memory: a ring per warp, and the warps' sums.
 __host__ __device__ constexpr int skinny_ring_bytes(int bits, int r, int ns) { return SKINNY_SLOTS * r * (256 * bits + 256 * ns); }
-__host__ __device__ constexpr int skinny_bytes(int bits, int nt, int r, int ns)
+__host__ __device__ constexpr int skinny_bytes(int bits, int r, int ns)
 {
-    return SKINNY_WARPS * ((ns < 4 ? skinny_ring_bytes(bits, r, ns) : 0) + 8 * nt * SKINNY_FEATS * r * 4);
+    return SKINNY_WARPS * ((ns < 4 ? skinny_ring_bytes(bits, r, ns) : 0) + SKINNY_ROWS * SKINNY_FEATS * r * 4);
 }
 
-// NT: rows of x in eights.  R: features of a block in sixteens.  NS: scales of a run, or 4: not regular.  A persistent CTA walks
+// R: features of a block in sixteens.  NS: scales of a run, or 4: not regular.  A persistent CTA walks
 // blocks of features (of each group of rows of each expert); codes of the next ones are on their way while one is finished.
 // `split`: warps that share a block's K.
-template <int KIND, int FDT, int NT, int R, int NS>
-__global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 && NT == 1 ? 3 : 2) linear_skinny_kernel(const LinearMmaArgs m)
+template <int KIND, int FDT, int R, int NS>
+__global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 ? 3 : 2) linear_skinny_kernel(const LinearMmaArgs m)
 {
-    constexpr int BITS = kind_bits(KIND), ROWS = 8 * NT, FEATS = SKINNY_FEATS * R, AHEAD = SKINNY_SLOTS - 1;
+    constexpr int BITS = kind_bits(KIND), ROWS = SKINNY_ROWS, FEATS = SKINNY_FEATS * R, AHEAD = SKINNY_SLOTS - 1;
     constexpr bool WHOLE = NS < 4;
     constexpr uint32_t CODES = R * 256 * BITS, SLOT = CODES + R * 256 * NS;   // 16 R rows of 128 codes, and their scales
     extern __shared__ __align__(128) uint8_t dyn[];
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 && NT == 1 ? 3 : 2) 
                   group * share * ROWS * FEATS;   // [warp][row][feature]
     const auto meet = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 * share) : "memory"); };
     pdl_entry();
-    const MmaSchedule sched = mma_schedule(m, reinterpret_cast<int *>(dyn + skinny_bytes(BITS, NT, R, NS)), 32 * SKINNY_WARPS);
+    const MmaSchedule sched = mma_schedule(m, reinterpret_cast<int *>(dyn + skinny_bytes(BITS, R, NS)), 32 * SKINNY_WARPS);
     const int groups = SKINNY_WARPS / share, first = blockIdx.x * groups + group, step = gridDim.x * groups, k = a.k, chunks = (k + 127) / 128;
     const uint32_t wide = a.param == QK_F32;
     const int scale_size = wide ? 4 : 2;
@@ -216,10 +216,8 @@ __global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 && NT == 1 ? 3 : 2) 
 #pragma unroll 1
     for (int t = first; t < sched.total; t += step) {
         const MmaTile tile = mma_tile(m, sched, t, FEATS);
-        const uint16_t *x0[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)   // rows past the tile repeat its last one; their sums are not stored
-            x0[n] = static_cast<const uint16_t *>(a.x) + (long long)(tile.r0 + min(8 * n + g, tile.rows - 1)) * a.x_stride + 32 * t4;
+        // rows past the tile repeat its last one; their sums are not stored
+        const uint16_t *x0 = static_cast<const uint16_t *>(a.x) + (long long)(tile.r0 + min(g, tile.rows - 1)) * a.x_stride + 32 * t4;
         uint32_t high = 0;   // which 16-bit scales are the high half of their word
         if (WHOLE && !wide) {
 #pragma unroll
@@ -227,7 +225,7 @@ __global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 && NT == 1 ? 3 : 2) 
 #pragma unroll
                 for (int j = 0; j < NS; ++j) high |= (uint32_t)(expert_scales(tile.e) + scale_offset(tile.f0 + 8 * i + g) + j * part_step >> 1 & 1) << (i * NS + j);
         }
-        float acc[R][NT][4] = {};
+        float acc[R][4] = {};
 #pragma unroll 1
         for (int c = warp; c < chunks; c += share) {
             const int col = c * 128 + 32 * t4, left = WHOLE ? 32 : codes_left(a, col);
@@ -268,20 +266,17 @@ __global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 && NT == 1 ? 3 : 2) 
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                uint32_t x[NT][8];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) fetch_x<WHOLE>(x[n], x0[n] + c * 128 + 16 * h, k - col - 16 * h);
+                uint32_t x[8];
+                fetch_x<WHOLE>(x, x0 + c * 128 + 16 * h, k - col - 16 * h);
                 if constexpr (split_pairs<KIND, NS>) {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int j = 0; j < 8; j += 4) {
-                            const uint32_t y0 = x[n][j], y1 = x[n][j + 1], y2 = x[n][j + 2], y3 = x[n][j + 3];
-                            x[n][j] = __byte_perm(y0, y2, 0x5410);
-                            x[n][j + 1] = __byte_perm(y0, y2, 0x7632);
-                            x[n][j + 2] = __byte_perm(y1, y3, 0x5410);
-                            x[n][j + 3] = __byte_perm(y1, y3, 0x7632);
-                        }
+                    for (int j = 0; j < 8; j += 4) {
+                        const uint32_t y0 = x[j], y1 = x[j + 1], y2 = x[j + 2], y3 = x[j + 3];
+                        x[j] = __byte_perm(y0, y2, 0x5410);
+                        x[j + 1] = __byte_perm(y0, y2, 0x7632);
+                        x[j + 2] = __byte_perm(y1, y3, 0x5410);
+                        x[j + 3] = __byte_perm(y1, y3, 0x7632);
+                    }
                 }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
@@ -292,9 +287,7 @@ __global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 && NT == 1 ? 3 : 2) 
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            mma_m16n8k16<FDT>(acc[r][n], o[0][2 * j], o[1][2 * j], o[0][2 * j + 1], o[1][2 * j + 1], x[n][2 * j], x[n][2 * j + 1]);
+                        mma_m16n8k16<FDT>(acc[r], o[0][2 * j], o[1][2 * j], o[0][2 * j + 1], o[1][2 * j + 1], x[2 * j], x[2 * j + 1]);
                 }
             }
             out += SLOT;
@@ -304,9 +297,7 @@ __global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 && NT == 1 ? 3 : 2) 
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) part[(warp * ROWS + 8 * n + 2 * t4 + (j & 1)) * FEATS + 16 * r + g + (j & 2) * 4] = acc[r][n][j];
+            for (int j = 0; j < 4; ++j) part[(warp * ROWS + 2 * t4 + (j & 1)) * FEATS + 16 * r + g + (j & 2) * 4] = acc[r][j];
         meet();
         for (int i = warp * 32 + lane; i < ROWS * FEATS; i += 32 * share) {
             const int r = i / FEATS, f = tile.f0 + i % FEATS;
@@ -322,25 +313,32 @@ __global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 && NT == 1 ? 3 : 2) 
 }
 
 // ---- launch -------------------------------------------------------------------------------------------------
-template <int KIND, int FDT, int NT, int R, int NS> static cudaError_t launch_skinny_rows(const LinearArgs &a, long long row_tiles, const LaunchCfg &cfg, cudaStream_t stream)
+// Time of a persistent grid in which groups of `split` warps take `tiles` blocks of 16 r features, in tenths of a warp's chunk of
+// 16 features: one of 32 takes 1.7 times as long, adding up a block's sums as long as a chunk.
+static long long skinny_time(long long tiles, long long ctas, int split, int chunks, int r)
+{
+    const long long groups = ctas * (SKINNY_WARPS / split);
+    return (tiles + groups - 1) / groups * ((chunks + split - 1) / split * (r == 2 ? 17 : 10) + 10);
+}
+
+template <int KIND, int FDT, int R, int NS>
+static cudaError_t launch_skinny_rows(const LinearArgs &a, long long row_tiles, int split, const LaunchCfg &cfg, cudaStream_t stream)
 {
     static std::atomic<unsigned long long> ready{0};
     LinearMmaArgs m = {};
     m.a = a;
-    m.tile_rows = 8 * NT;
+    m.tile_rows = SKINNY_ROWS;
     m.feat_tiles = (a.feats + SKINNY_FEATS * R - 1) / (SKINNY_FEATS * R);
     m.by_feat_tiles = make_fastdiv((unsigned)m.feat_tiles);
-    const long long tiles = row_tiles * m.feat_tiles, resident = cfg.sm_count * (NS < 4 && NT == 1 ? 3 : 2);
+    const long long tiles = row_tiles * m.feat_tiles, resident = cfg.sm_count * (NS < 4 ? 3 : 2);
     if (tiles >= (1ll << 31)) return cudaErrorInvalidConfiguration;
-    // as few warps to a block as leave four blocks for each group (fewer sums to add, fewer barriers), but no more than chunks
-    m.split = SKINNY_WARPS;
-    while (m.split > 2 && (tiles >= 4 * resident * SKINNY_WARPS * 2 / m.split || m.split > (a.k + 127) / 128)) m.split /= 2;
-    const size_t smem = skinny_bytes(kind_bits(KIND), NT, R, NS) + (a.offsets ? (3 * a.experts + 1) * 4 : 0);
+    m.split = split;
+    const size_t smem = skinny_bytes(kind_bits(KIND), R, NS) + (a.offsets ? (3 * a.experts + 1) * 4 : 0);
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !(ready.load(std::memory_order_acquire) >> dev & 1)) {   // devices whose shared-memory limit of this kernel is raised
-        e = cudaFuncSetAttribute(linear_skinny_kernel<KIND, FDT, NT, R, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+        e = cudaFuncSetAttribute(linear_skinny_kernel<KIND, FDT, R, NS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
     }
@@ -355,25 +353,38 @@ template <int KIND, int FDT, int NT, int R, int NS> static cudaError_t launch_sk
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     c.attrs = attr;
     c.numAttrs = cfg.pdl ? 1 : 0;
-    return cudaLaunchKernelEx(&c, linear_skinny_kernel<KIND, FDT, NT, R, NS>, m);
-}
-
-template <int KIND, int FDT, int NT> static cudaError_t launch_skinny_nt(const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
-{
-    long long row_tiles = (a.rows + 8 * NT - 1) / (8 * NT);
-    if (a.offsets) row_tiles += a.experts < a.rows ? a.experts : a.rows;   // at most
-    const int scales = skinny_regular(a) ? a.run_scales : 4;
-    // 32 features a block where that leaves a block for every resident CTA: x is fetched half as often
-    const bool tall = scales < 4 && row_tiles * (a.feats / 32) >= 3ll * cfg.sm_count;
-    if (scales == 4) return launch_skinny_rows<KIND, FDT, NT, 1, 4>(a, row_tiles, cfg, stream);
-    if (scales == 1)
-        return tall ? launch_skinny_rows<KIND, FDT, NT, 2, 1>(a, row_tiles, cfg, stream) : launch_skinny_rows<KIND, FDT, NT, 1, 1>(a, row_tiles, cfg, stream);
-    return tall ? launch_skinny_rows<KIND, FDT, NT, 2, 2>(a, row_tiles, cfg, stream) : launch_skinny_rows<KIND, FDT, NT, 1, 2>(a, row_tiles, cfg, stream);
+    return cudaLaunchKernelEx(&c, linear_skinny_kernel<KIND, FDT, R, NS>, m);
 }
 
 template <int KIND, int FDT> static cudaError_t launch_skinny_one(const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
 {
-    return a.rows <= 8 * a.experts ? launch_skinny_nt<KIND, FDT, 1>(a, cfg, stream) : launch_skinny_nt<KIND, FDT, 2>(a, cfg, stream);
+    const int scales = skinny_regular(a) ? a.run_scales : 4, chunks = (a.k + 127) / 128;
+    const long long busy = a.experts < a.rows ? a.experts : a.rows;   // experts with rows, at most
+    long long row_tiles = (a.rows + SKINNY_ROWS - 1) / SKINNY_ROWS, expected = row_tiles;
+    if (a.offsets) {
+        row_tiles += busy;   // at most
+        expected = busy + a.rows / 32;
+    }
+    // 16 or 32 features a block, 8, 4 or 2 warps to one
+    const long long ctas = (long long)cfg.sm_count * (scales < 4 ? 3 : 2);
+    int best_r = 1, split = SKINNY_WARPS;
+    long long best = 0;
+    for (int r = scales < 4 ? 2 : 1; r >= 1; --r) {
+        for (int w = SKINNY_WARPS; w >= 2; w /= 2) {
+            const long long time = skinny_time(expected * ((a.feats + 16 * r - 1) / (16 * r)), ctas, w, chunks, r);
+            if (best == 0 || time < best) {
+                best = time;
+                best_r = r;
+                split = w;
+            }
+        }
+    }
+    if (scales == 4) return launch_skinny_rows<KIND, FDT, 1, 4>(a, row_tiles, split, cfg, stream);
+    if (scales == 1)
+        return best_r == 2 ? launch_skinny_rows<KIND, FDT, 2, 1>(a, row_tiles, split, cfg, stream)
+                           : launch_skinny_rows<KIND, FDT, 1, 1>(a, row_tiles, split, cfg, stream);
+    return best_r == 2 ? launch_skinny_rows<KIND, FDT, 2, 2>(a, row_tiles, split, cfg, stream)
+                       : launch_skinny_rows<KIND, FDT, 1, 2>(a, row_tiles, split, cfg, stream);
 }
 
 template <int FDT> static cudaError_t launch_skinny_kind(int kind, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
