@@ -218,11 +218,11 @@ __device__ __forceinline__ void decode_code_run(const LinearArgs &a, const CodeR
 
 // Runs on their way from memory where they cannot be fetched as tiles: a thread copies its own ones to its own places in
 // shared memory by asynchronous copies of 16, 8 or 4 bytes, several steps ahead, and nothing but the thread itself waits for
-// them.
+// them.  Rows that start on no word are copied with the words that hold them, one more than a run has.
 template <int KIND> struct StagedRuns {
     static constexpr int WORDS = CodeRun<KIND>::WORDS;
-    static constexpr int AHEAD = WORDS >= 8 ? 2 : WORDS >= 4 ? 3 : 4;
-    __host__ __device__ static constexpr int slot_bytes(int threads) { return threads * (WORDS * 4 + 16); }
+    static constexpr int AHEAD = WORDS >= 4 ? 2 : 3;
+    __host__ __device__ static constexpr int slot_bytes(int threads) { return threads * (WORDS * 4 + 20); }
 };
 
 __device__ __forceinline__ void copy_async16(uint32_t dst, const void *src, int bytes)
@@ -257,21 +257,14 @@ __device__ __forceinline__ void stage_code_run(const LinearArgs &a, uint32_t slo
                 copy_async16(slot + (i * threads + id) * 16, left > 0 ? p + 16 * i : a.codes, left < 0 ? 0 : left > 16 ? 16 : left);
             }
         }
-    } else if (a.code_align >= 4) {
-        const uint8_t *none = reinterpret_cast<const uint8_t *>((uintptr_t)a.codes & ~(uintptr_t)3);
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) {
-            const uint32_t dst = WORDS == 2 ? slot + id * 8 + i * 4 : slot + ((i / 4) * threads + id) * 16 + (i % 4) * 4;
-            const int left = min(bytes - 4 * i, 4);
-            copy_async4(dst, left > 0 ? p + 4 * i : none, left > 0 ? left : 0);
-        }
     } else {
-#pragma unroll 1
-        for (int i = 0; i < WORDS; ++i) {
-            const uint32_t dst = WORDS == 2 ? slot + id * 8 + i * 4 : slot + ((i / 4) * threads + id) * 16 + (i % 4) * 4;
-            uint32_t v = 0;
-            for (int j = 0; j < 4 && 4 * i + j < bytes; ++j) v |= (uint32_t)__ldg(p + 4 * i + j) << (8 * j);
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(v) : "memory");
+        const uintptr_t word = reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3, none = reinterpret_cast<uintptr_t>(a.codes) & ~(uintptr_t)3;
+        const int span = valid ? (int)(reinterpret_cast<uintptr_t>(p) - word) + bytes : 0;   // bytes from the first word to the run's end
+#pragma unroll
+        for (int i = 0; i <= WORDS; ++i) {
+            const uint32_t dst = i == WORDS ? slot + threads * (WORDS * 4 + 16) + id * 4
+                                            : WORDS == 2 ? slot + id * 8 + i * 4 : slot + ((i / 4) * threads + id) * 16 + (i % 4) * 4;
+            if (i < WORDS || a.code_align < 4) copy_async4(dst, reinterpret_cast<const void *>(span > 4 * i ? word + 4 * i : none), span > 4 * i ? 4 : 0);
         }
     }
     const uint32_t scales = slot + threads * WORDS * 4 + id * 4;
@@ -285,8 +278,8 @@ __device__ __forceinline__ void stage_code_run(const LinearArgs &a, uint32_t slo
     }
 }
 
-// The codes of a staged run, once its copies have arrived.
-template <int KIND> __device__ __forceinline__ void take_codes(CodeRun<KIND> &r, uint32_t slot, int id, int threads)
+// The codes of a staged run, once its copies have arrived; it starts `skip` bytes into its first word.
+template <int KIND> __device__ __forceinline__ void take_codes(CodeRun<KIND> &r, uint32_t slot, int id, int threads, unsigned skip)
 {
     constexpr int WORDS = CodeRun<KIND>::WORDS;
     if constexpr (WORDS == 2) {
@@ -298,6 +291,12 @@ template <int KIND> __device__ __forceinline__ void take_codes(CodeRun<KIND> &r,
                          : "=r"(r.w[i]), "=r"(r.w[i + 1]), "=r"(r.w[i + 2]), "=r"(r.w[i + 3])
                          : "r"(slot + (i / 4 * threads + id) * 16)
                          : "memory");
+    }
+    if (skip != 0) {
+        uint32_t last;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(last) : "r"(slot + threads * (WORDS * 4 + 16) + id * 4) : "memory");
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) r.w[i] = __funnelshift_r(r.w[i], i + 1 < WORDS ? r.w[i + 1] : last, 8 * skip);
     }
 }
 // A scale staged at shared address `from`; `at`: its address in memory (of which the last bits say where in the word it is).

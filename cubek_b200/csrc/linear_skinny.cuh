@@ -19,19 +19,16 @@ namespace qk {
 template <int KIND> __device__ __forceinline__ void fetch_run(const LinearArgs &a, CodeRun<KIND> &r, const CodeRow &row, int col)
 {
     constexpr int BITS = CodeRun<KIND>::BITS, WORDS = CodeRun<KIND>::WORDS;
+    // the words that hold the run, and what lies in them before it shifted out
     const int valid = row.exists ? codes_left(a, col) : 0, bytes = (valid * BITS + 7) / 8;
-    const uint8_t *p = row.codes + (long long)col * BITS / 8;
+    const uintptr_t p = reinterpret_cast<uintptr_t>(row.codes) + (long long)col * BITS / 8, word = p & ~(uintptr_t)3;
+    const unsigned skip = (unsigned)(p - word);
+    uint32_t raw[WORDS + 1];
 #pragma unroll
-    for (int i = 0; i < WORDS; ++i) {
-        r.w[i] = 0;
-        if (a.code_align >= 4 && 4 * i + 4 <= bytes) {
-            r.w[i] = __ldg(reinterpret_cast<const uint32_t *>(p) + i);
-        } else {
+    for (int i = 0; i <= WORDS; ++i)
+        raw[i] = valid && (int)skip + bytes > 4 * i ? __ldg(reinterpret_cast<const uint32_t *>(word) + i) : 0u;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (4 * i + j < bytes) r.w[i] |= (uint32_t)__ldg(p + 4 * i + j) << (8 * j);
-        }
-    }
+    for (int i = 0; i < WORDS; ++i) r.w[i] = __funnelshift_r(raw[i], raw[i + 1], 8 * skip);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         r.s[i] = 0;

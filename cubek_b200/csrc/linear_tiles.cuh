@@ -26,7 +26,7 @@ struct LinearMmaArgs {
 };
 
 constexpr int MMA_MAX_STAGES = 8;
-constexpr int MMA_SMEM_LIMIT = 225 * 1024;   // dynamic; the barriers are static
+constexpr int MMA_SMEM_LIMIT = 451 * 512;   // dynamic, of 227 KiB; the barriers are static
 
 struct MmaTile {
     int e, f0, r0, rows;
@@ -118,7 +118,7 @@ constexpr int WEIGHT_THREADS = 128, WEIGHT_GROUPS = 4, WEIGHT_SCALES_AHEAD = 4;
 __host__ __device__ constexpr int weight_bytes(int kind, int scales, int slots)
 {
     return scales == 0 ? WEIGHT_GROUPS * (kind_bits(kind) == 8 ? StagedRuns<KIND_I8>::AHEAD : kind_bits(kind) == 4 ? StagedRuns<KIND_PACK4>::AHEAD : StagedRuns<KIND_PACK2>::AHEAD) * WEIGHT_THREADS *
-                             (kind_bits(kind) * 4 + 16)
+                             (kind_bits(kind) * 4 + 20)
                        : slots * 512 * kind_bits(kind) + WEIGHT_GROUPS * WEIGHT_SCALES_AHEAD * WEIGHT_THREADS * 4 * scales;
 }
 
@@ -286,7 +286,10 @@ template <int KIND, int FDT, bool BWD, int STRIDE, int SLOTS> struct WeightWarps
                     uint32_t o[16];
                     const int col = BWD ? features(tile) + run_col : kb * 64 + run_col;
                     if (BWD && a.param != QK_F32) row = code_row(a, tile.e, kb * 64 + r);
-                    take_codes<KIND>(run, out_slot, id, WEIGHT_THREADS);
+                    const unsigned skip =
+                        a.code_align >= 4 ? 0u : 3u & ((unsigned)reinterpret_cast<uintptr_t>(a.codes) + (unsigned)tile.e * (unsigned)a.code_expert +
+                                                       (unsigned)(BWD ? kb * 64 + r : features(tile) + r) * (unsigned)a.code_row);
+                    take_codes<KIND>(run, out_slot, id, WEIGHT_THREADS, skip);
                     const uint32_t from = out_slot + WEIGHT_THREADS * CodeRun<KIND>::WORDS * 4 + id * 4;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
