@@ -162,7 +162,7 @@ static int run_product(int dtype, const QkScheme *s, bool backward, LinearArgs &
                (!a.pre || rows_on(bytes, a.pre, a.pre_stride));
     };
     a.pairs = a.feats % 2 == 0 && all_on(4);
-    a.wide = all_on(32);
+    a.wide = all_on(32) ? 32 : all_on(16) ? 16 : 0;
     a.error_flag = stage_error_flag();
     count_launch();
     return cuda_status(launch_linear_product(dtype, kind_of(s), backward, a, current_cfg(), stream));

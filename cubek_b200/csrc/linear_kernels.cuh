@@ -39,7 +39,7 @@ struct LinearArgs {
     long long pre_stride;
     int act;                          // QkActivation
     int pairs;                        // two neighbouring features may be read and written as one 32-bit word,
-    int wide;                         // 16 of them as 32 bytes
+    int wide;                         // 16 of them as 32 bytes (32) or twice 16 (16); 0: neither
     // experts
     const void *offsets;              // nullptr: one expert with all rows
     int offsets64;

@@ -54,8 +54,9 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     m.by_feat_tiles = make_fastdiv((unsigned)m.feat_tiles);
     m.split = 1;
     // Pairs of CTAs from 160 rows (of an expert, on average).  8 experts 14336 x 4096 q4 with 128, 192, 256 rows: 277, 293,
-    // 303 us, the other kernel 256, 298, 336; one 4096 x 4096: 27, 27, 27 and 25, 29, 33.
-    const bool wide = average >= 160 && m.kblocks > 0;
+    // 303 us, the other kernel 256, 298, 336; one 4096 x 4096: 27, 27, 27 and 25, 29, 33.  They store a row's features
+    // from one lane, which rows that start on no 16 bytes would turn into single elements all over memory.
+    const bool wide = average >= 160 && m.kblocks > 0 && a.wide;
     long long row_tiles;
     if (wide) {
         m.tile_rows = WIDE_ROWS;

@@ -25,16 +25,21 @@ template <int FDT> __device__ __forceinline__ void wide_store16(const LinearArgs
     using F = typename ElemOf<FDT>::type;
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] += bias[i];
-    const bool whole = a.wide && f + 16 <= a.feats;
+    const bool whole = f + 16 <= a.feats;
     const auto put = [&](void *base, long long stride) {
         F *p = static_cast<F *>(base) + row * stride + f;
         if (whole) {
             uint32_t o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = h2_pack<FDT>(v[2 * i], v[2 * i + 1]);
-            asm volatile("st.global.v8.u32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]),
-                         "r"(o[6]), "r"(o[7])
-                         : "memory");
+            if (a.wide == 32) {
+                asm volatile("st.global.v8.u32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]),
+                             "r"(o[5]), "r"(o[6]), "r"(o[7])
+                             : "memory");
+            } else {
+                reinterpret_cast<uint4 *>(p)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                reinterpret_cast<uint4 *>(p)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -47,10 +52,14 @@ template <int FDT> __device__ __forceinline__ void wide_store16(const LinearArgs
         const F *p = static_cast<const F *>(a.residual) + row * a.residual_stride + f;
         if (whole) {
             uint32_t q[8];
-            asm volatile("ld.global.v8.u32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                         : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7])
-                         : "l"(p)
-                         : "memory");
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint4 u = reinterpret_cast<const uint4 *>(p)[i];
+                q[4 * i] = u.x;
+                q[4 * i + 1] = u.y;
+                q[4 * i + 2] = u.z;
+                q[4 * i + 3] = u.w;
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 v[2 * i] += widen_lo<FDT>(q[i]);
