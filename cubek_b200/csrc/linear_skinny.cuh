@@ -310,14 +310,6 @@ __global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 ? 3 : 2) linear_skin
 }
 
 // ---- launch -------------------------------------------------------------------------------------------------
-// Time of a persistent grid in which groups of `split` warps take `tiles` blocks of 16 r features, in tenths of a warp's chunk of
-// 16 features: one of 32 takes 1.7 times as long, adding up a block's sums as long as a chunk.
-static long long skinny_time(long long tiles, long long ctas, int split, int chunks, int r)
-{
-    const long long groups = ctas * (SKINNY_WARPS / split);
-    return (tiles + groups - 1) / groups * ((chunks + split - 1) / split * (r == 2 ? 17 : 10) + 10);
-}
-
 template <int KIND, int FDT, int R, int NS>
 static cudaError_t launch_skinny_rows(const LinearArgs &a, long long row_tiles, int split, const LaunchCfg &cfg, cudaStream_t stream)
 {
@@ -362,20 +354,15 @@ template <int KIND, int FDT> static cudaError_t launch_skinny_one(const LinearAr
         row_tiles += busy;   // at most
         expected = busy + a.rows / 32;
     }
-    // 16 or 32 features a block, 8, 4 or 2 warps to one
+    // 32 features a block (x is fetched half as often) where that leaves three blocks for each CTA and three CTAs fit an SM,
+    // which those of 8-bit codes do not; else 16.  Four warps to a block where eight leave each CTA eight blocks (half as
+    // many sums to add); fewer where K has fewer chunks.  One row, 14336 x 4096 q4, 16 features and 8 warps (3 rounds) 19 us, 32 and
+    // 4 (1 round) 26; one row for each of 8 experts, 32 and 4 (5 rounds) 59 us, 32 and 8 (9 rounds) 69.
     const long long ctas = (long long)cfg.sm_count * (scales < 4 ? 3 : 2);
-    int best_r = 1, split = SKINNY_WARPS;
-    long long best = 0;
-    for (int r = scales < 4 ? 2 : 1; r >= 1; --r) {
-        for (int w = SKINNY_WARPS; w >= 2; w /= 2) {
-            const long long time = skinny_time(expected * ((a.feats + 16 * r - 1) / (16 * r)), ctas, w, chunks, r);
-            if (best == 0 || time < best) {
-                best = time;
-                best_r = r;
-                split = w;
-            }
-        }
-    }
+    const auto blocks = [&](int r) { return expected * ((a.feats + 16 * r - 1) / (16 * r)); };
+    const int best_r = scales < 4 && kind_bits(KIND) < 8 && blocks(2) > 2 * ctas ? 2 : 1;
+    int split = blocks(best_r) > 7 * ctas ? 4 : 8;
+    while (split > 2 && split / 2 >= chunks) split /= 2;
     if (scales == 4) return launch_skinny_rows<KIND, FDT, 1, 4>(a, row_tiles, split, cfg, stream);
     if (scales == 1)
         return best_r == 2 ? launch_skinny_rows<KIND, FDT, 2, 1>(a, row_tiles, split, cfg, stream)
