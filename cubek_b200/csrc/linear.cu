@@ -62,7 +62,7 @@ static int fill_weight(LinearArgs &a, const QkTensor *values, const QkTensor *pa
     if (values->rank != r) return QK_ERR_SHAPE;
     const long long e = grouped ? values->shape[0] : 1, n = values->shape[r - 2], items = values->shape[r - 1], k = items * nq;
     if (grouped && e < 1) return QK_ERR_SHAPE;
-    if (n >= (1ll << 30) || k >= (1ll << 30) || e > QK_LINEAR_MAX_EXPERTS) return QK_ERR_TOO_LARGE;
+    if (n >= QK_LINEAR_MAX_EXTENT || k >= QK_LINEAR_MAX_EXTENT || e > QK_LINEAR_MAX_EXPERTS) return QK_ERR_TOO_LARGE;
     a.experts = (int)e;
     a.n = (int)n;
     a.k = (int)k;

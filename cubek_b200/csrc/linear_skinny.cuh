@@ -47,7 +47,7 @@ template <bool WHOLE> __device__ __forceinline__ void fetch_x(uint32_t *x, const
     for (int i = 0; i < 2; ++i) {
         if (WHOLE || left <= 8 * i || left >= 8 * i + 8) {
             const uint32_t ok = left > 8 * i;
-            asm("{\n.reg .pred p;\nsetp.ne.u32 p, %5, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\nmov.b32 %2, 0;\nmov.b32 %3, 0;\n"
+            asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %5, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\nmov.b32 %2, 0;\nmov.b32 %3, 0;\n"
                 "@p ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
                          : "=&r"(x[4 * i]), "=&r"(x[4 * i + 1]), "=&r"(x[4 * i + 2]), "=&r"(x[4 * i + 3])
                          : "l"(p + 8 * i), "r"(ok));
@@ -226,6 +226,9 @@ __global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 ? 3 : 2) linear_skin
 #pragma unroll 1
         for (int c = warp; c < chunks; c += share) {
             const int col = c * 128 + 32 * t4, left = WHOLE ? 32 : codes_left(a, col);
+            uint32_t xs[2][8];   // on their way while the codes are waited for
+#pragma unroll
+            for (int h = 0; h < 2; ++h) fetch_x<WHOLE>(xs[h], x0 + c * 128 + 16 * h, k - col - 16 * h);
             CodeRun<KIND> q[2 * R];
             if constexpr (WHOLE) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
@@ -263,8 +266,7 @@ __global__ void __launch_bounds__(32 * SKINNY_WARPS, NS < 4 ? 3 : 2) linear_skin
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                uint32_t x[8];
-                fetch_x<WHOLE>(x, x0 + c * 128 + 16 * h, k - col - 16 * h);
+                uint32_t *x = xs[h];
                 if constexpr (split_pairs<KIND, NS>) {
 #pragma unroll
                     for (int j = 0; j < 8; j += 4) {
@@ -364,10 +366,12 @@ template <int KIND, int FDT> static cudaError_t launch_skinny_one(const LinearAr
     int split = blocks(best_r) > 7 * ctas ? 4 : 8;
     while (split > 2 && split / 2 >= chunks) split /= 2;
     if (scales == 4) return launch_skinny_rows<KIND, FDT, 1, 4>(a, row_tiles, split, cfg, stream);
-    if (scales == 1)
-        return best_r == 2 ? launch_skinny_rows<KIND, FDT, 2, 1>(a, row_tiles, split, cfg, stream)
-                           : launch_skinny_rows<KIND, FDT, 1, 1>(a, row_tiles, split, cfg, stream);
-    return best_r == 2 ? launch_skinny_rows<KIND, FDT, 2, 2>(a, row_tiles, split, cfg, stream)
+    if constexpr (kind_bits(KIND) < 8) {
+        if (best_r == 2)
+            return scales == 1 ? launch_skinny_rows<KIND, FDT, 2, 1>(a, row_tiles, split, cfg, stream)
+                               : launch_skinny_rows<KIND, FDT, 2, 2>(a, row_tiles, split, cfg, stream);
+    }
+    return scales == 1 ? launch_skinny_rows<KIND, FDT, 1, 1>(a, row_tiles, split, cfg, stream)
                        : launch_skinny_rows<KIND, FDT, 1, 2>(a, row_tiles, split, cfg, stream);
 }
 

@@ -322,7 +322,8 @@ inline void mma_steps(LinearMmaArgs &m, bool backward, int stride)
     const unsigned block = backward ? a.bn.div : a.bk.div;
     const long long scale_step = backward ? a.scale_row : a.scale_col;
     const bool one = scale_step == 0;
-    m.regular = a.code_align == 16 && a.k % 32 == 0 && a.contraction % 64 == 0 && a.run_scales <= 2 && (one || rows % block == 0);
+    // two scales of a run are neighbours in blocks of 16 alone: of 48, one run has both halves in one block
+    m.regular = a.code_align == 16 && a.k % 32 == 0 && a.contraction % 64 == 0 && (a.run_scales == 1 || a.bk.div == 16) && (one || rows % block == 0);
     m.scale_step = one ? 0 : rows / block * scale_step * size;
 }
 

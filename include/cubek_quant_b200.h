@@ -303,8 +303,11 @@ int qk_into_contiguous_packed(const QkTensor *input, const QkTensor *output, con
  *   residual  [.., N], typed as x; NULL: none; may be the output itself
  *   output    y [.., N], typed as x; overlaps no input but `residual`
  *   pre       [.., N], receives x W^T + bias (rounded), which the gradient of the activation needs; NULL: not kept
- * A column-major operand (packed along N) is QK_ERR_LAYOUT: qk_into_contiguous_packed makes it row-major.
+ * A column-major operand (packed along N) is QK_ERR_LAYOUT: qk_into_contiguous_packed makes it row-major.  N and K are
+ * below QK_LINEAR_MAX_EXTENT (a sum of that length takes the tensor cores half a second, and their waits end after
+ * two), rows below 2^31.  As with the other entry points, make the first call on a device before any stream capture.
  */
+#define QK_LINEAR_MAX_EXTENT (1ll << 26)
 typedef enum {
     QK_ACT_IDENTITY = 0, QK_ACT_RELU = 1, QK_ACT_GELU = 2 /* z Phi(z) */, QK_ACT_GELU_TANH = 3 /* its tanh form */, QK_ACT_SILU = 4
 } QkActivation;
@@ -354,7 +357,8 @@ const char *qk_version(void);
 
 /* Reads AND CLEARS (synchronously: the call waits for the device) the error flag of the current device: `*flag_out`
  * is non-zero if, since the last call, a kernel gave up on a bounded wait and left its output unwritten.  Only the
- * quantize variant that stages its input through shared memory with bulk copies has such waits.  Entry points
+ * quantize variant that stages its input through shared memory with bulk copies and the products with quantized weights
+ * have such waits.  Entry points
  * are asynchronous and cannot report this themselves: callers that need the guarantee call this after
  * synchronising the stream.  qk_roundtrip_host, which synchronises anyway, checks the flag itself and returns
  * QK_ERR_DEVICE. */

@@ -118,6 +118,16 @@ def test_grouped():
     assert status(back, Y, off, w, X, BF, activation=Activation.Relu) == _ffi.QK_ERR_NULL
 
 
+def test_extents():
+    wide = weight((8, 1 << 26))
+    assert status(linear.launch, fake((1, 1 << 26), 2), wide, fake((1, 8), 2), BF) == _ffi.QK_ERR_TOO_LARGE
+    tall = weight((1 << 26, 32))
+    assert status(linear.launch, fake((1, 32), 2), tall, fake((1, 1 << 26), 2), BF) == _ffi.QK_ERR_TOO_LARGE
+    assert status(linear.launch_backward, fake((1, 1 << 26), 2), tall, fake((1, 32), 2), BF) == _ffi.QK_ERR_TOO_LARGE
+    with pytest.raises(LaunchError):   # an unaligned x needs the workspace
+        linear.launch(CLIENT, fake((20, 64), 2, addr=0x10002), weight(), fake((20, 64), 2), BF)
+
+
 def test_null_arguments():
     x, v, p = _ffi.c_tensors(X, fake((64, 8), 4), fake((64, 2), 4))
     s = _ffi.c_scheme(Q4)
