@@ -187,32 +187,33 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1) linear_narrow_kernel(const 
         }
     } else if (warp == 5) {
         // ---- products -----------------------------------------------------------------------------------
-        const uint32_t idesc = instr_desc(FDT == QK_BF16, BWD, 128, m.tile_rows);
+        const uint32_t idesc = instr_desc(FDT == QK_BF16, BWD, 128, m.tile_rows), stage_step = stage_bytes / 16;
+        // K-major: 16 steps are 32 bytes of a swizzled row.  MN-major: two groups of 8 rows of 128 bytes.
+        const uint64_t da0 = BWD ? smem_desc(base, 8192, 1024) : smem_desc(base, 16, 1024), db0 = smem_desc(base + A_BYTES, 16, 1024);
         int buf = 0, buf_phase = 0;
         for (int t = first; t < sched.total; t += step) {
             if (kb0 < kb1) {
                 wait(acc_empty(buf), buf_phase ^ 1);
                 tc_fence_after();
                 const uint32_t d = tmem + buf * m.tile_rows;
+                // What a step costs here bounds few rows: descriptors are made once, and a step adds to them.
 #pragma unroll 1
                 for (int kb = kb0; kb < kb1; ++kb) {
                     wait(full(stage), phase);
-                    dead = __any_sync(0xffffffffu, dead);
-                    if (dead) break;
+                    if (__any_sync(0xffffffffu, dead)) break;
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t sa = base + stage * stage_bytes;
-                        // K-major: 16 steps are 32 bytes of a swizzled row.  MN-major: two groups of 8 rows of 128 bytes.
-                        const uint64_t da = BWD ? smem_desc(sa, 8192, 1024) : smem_desc(sa, 16, 1024), db = smem_desc(sa + A_BYTES, 16, 1024);
+                        const uint32_t at = (uint32_t)stage * stage_step;
+                        mma_f16<1>(d, da0 + at, db0 + at, idesc, kb > kb0);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            mma_f16<1>(d, da + i * (BWD ? 2048 / 16 : 32 / 16), db + i * (32 / 16), idesc, kb > kb0 || i > 0);
+                        for (int i = 1; i < 4; ++i) mma_f16<1>(d, da0 + at + i * (BWD ? 2048 / 16 : 32 / 16), db0 + at + i * (32 / 16), idesc, true);
                         mma_commit<1>(empty(stage));
-                        if (kb == kb1 - 1) mma_commit<1>(acc_full(buf));
                     }
                     __syncwarp();
                     next_stage();
                 }
+                if (elect_one()) mma_commit<1>(acc_full(buf));
+                __syncwarp();
                 buf ^= 1;
                 if (buf == 0) buf_phase ^= 1;
             }
