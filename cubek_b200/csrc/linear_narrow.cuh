@@ -229,24 +229,28 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1) linear_narrow_kernel(const 
         __syncwarp();
     } else if (warp == 6) {
         // ---- tiles of codes -------------------------------------------------------------------------------
-        constexpr int SLOTS = NARROW_SLOTS, BITS = kind_bits(KIND), TILE_BYTES = 512 * BITS;
-        int slot = 0, slot_phase = 0, started = 0;
+        // Lane l serves group l of the weight: its half of every other step, its slots.  (One lane for all of them took 1000
+        // cycles a step, which the groups waited for.)
+        constexpr int BITS = kind_bits(KIND), TILE_BYTES = 512 * BITS;
+        int slot = lane, slot_phase = 0, started = 0, kb = kb0 + lane / 2;
         for (int t = first; t < sched.total; t += step) {
             const MmaTile tile = mma_tile(m, sched, t, NARROW_FEATS);
-            if (lane == 0 && m.regular) {
+            if (lane < WEIGHT_GROUPS && m.regular && kb0 < kb1) {
+                const int f = tile.f0 + (lane & 1) * 64;
 #pragma unroll 1
-                for (int u = 2 * kb0; u < 2 * kb1; ++u) {   // two halves of 64 features a step
-                    const int kb = u / 2, f = tile.f0 + (u & 1) * 64;
+                for (; kb < kb1; kb += 2) {
                     wait(codes_empty(slot), slot_phase ^ 1);
-                    if (dead) break;
+                    if (dead) continue;
                     mbar_expect_tx(codes_full(slot), TILE_BYTES);
                     tma_load_3d(runs + slot * TILE_BYTES, &wmap, (BWD ? f : kb * 64) * BITS / 8, BWD ? kb * 64 : f, tile.e, codes_full(slot));
                     ++started;
-                    if (++slot == SLOTS) {
-                        slot = 0;
+                    slot += WEIGHT_GROUPS;
+                    if (slot >= NARROW_SLOTS) {
+                        slot -= NARROW_SLOTS;
                         slot_phase ^= 1;
                     }
                 }
+                kb -= kb1 - kb0;
             }
             if (m.split > 1) {
                 meet();
@@ -255,9 +259,12 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1) linear_narrow_kernel(const 
             }
         }
         if (dead) {
-            for (int i = min(started, SLOTS); i > 0; --i) {
-                slot = slot == 0 ? SLOTS - 1 : slot - 1;
-                if (slot == SLOTS - 1) slot_phase ^= 1;
+            for (int i = min(started, NARROW_SLOTS / WEIGHT_GROUPS); i > 0; --i) {
+                slot -= WEIGHT_GROUPS;
+                if (slot < 0) {
+                    slot += NARROW_SLOTS;
+                    slot_phase ^= 1;
+                }
                 mbar_wait(codes_full(slot), slot_phase, nullptr);
             }
         }
