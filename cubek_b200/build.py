@@ -46,6 +46,7 @@ def _stale(target: Path, deps) -> bool:
 
 
 def _compile(src: Path, verbose: bool, half_away: bool = False) -> Path:
+    half_away = half_away and not src.stem.startswith("linear")   # the products round no quotient: one object for both
     obj = BUILD / (src.stem + (".half_away.o" if half_away else ".o"))
     if _stale(obj, [src, *_headers()]):
         cmd = [NVCC, *NVCC_FLAGS, *(["-DQK_ROUND_HALF_AWAY"] if half_away else []), "-c", str(src), "-o", str(obj)]

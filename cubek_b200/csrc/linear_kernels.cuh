@@ -79,7 +79,15 @@ __device__ __forceinline__ float normal_cdf(float z, float &bell)
 {
     const float t = __fdividef(1.0f, fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.0f));
     bell = __expf(-0.5f * z * z);
-    const float tail = 0.5f * bell * t * fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(fmaf(-0.141663104f, t, 0.498880595f), t, -0.409603357f), t, 0.456564605f), t, 0.023715185f), t, 0.206398115f), t, 0.180649981f), t, 0.185058087f);
+    float p = -0.141663104f;
+    p = fmaf(p, t, 0.498880595f);
+    p = fmaf(p, t, -0.409603357f);
+    p = fmaf(p, t, 0.456564605f);
+    p = fmaf(p, t, 0.023715185f);
+    p = fmaf(p, t, 0.206398115f);
+    p = fmaf(p, t, 0.180649981f);
+    p = fmaf(p, t, 0.185058087f);
+    const float tail = 0.5f * bell * t * p;
     return z < 0.0f ? tail : 1.0f - tail;
 }
 

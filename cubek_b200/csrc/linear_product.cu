@@ -53,9 +53,9 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     m.feat_tiles = (a.feats + 127) / 128;
     m.by_feat_tiles = make_fastdiv((unsigned)m.feat_tiles);
     m.split = 1;
-    // Pairs of CTAs from 160 rows (of an expert, on average).  8 experts 14336 x 4096 q4 with 128, 192, 256 rows: 277, 293,
-    // 303 us, the other kernel 256, 298, 336; one 4096 x 4096: 27, 27, 27 and 25, 29, 33.  They store a row's features
-    // from one lane, which rows that start on no 16 bytes would turn into single elements all over memory.
+    // Pairs of CTAs from 160 rows (of an expert, on average): 8 experts 14336 x 4096 q4 with 128 and 159 rows on the other kernel
+    // 264 and 270 us, 128 and 192 rows on pairs 277 and 293; one 4096 x 4096 with 159 rows 27, on pairs 27.  Pairs store a row's
+    // features from one lane, which rows that start on no 16 bytes would turn into single elements all over memory.
     const bool wide = average >= 160 && m.kblocks > 0 && a.wide;
     long long row_tiles;
     if (wide) {
@@ -121,8 +121,8 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
 
 cudaError_t launch_linear_product(int fdt, int kind, bool backward, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
 {
-    // A handful of rows (of an expert, on average): 14336 x 4096 q8 with 8 rows 21 us, 16 rows on the tiles of the tensor
-    // cores 36; with 8 experts 223 and 232.
+    // A handful of rows (of an expert, on average): 14336 x 4096 q8 with 8 rows 22 us, with 9 on the tiles of the tensor
+    // cores 31; of each of 8 experts, q4, 148 and 202 us, q8 both 195.
     if (!backward && a.k > 0 && a.rows <= 8 * a.experts)
         return fdt == QK_F16 ? launch_skinny_f16(kind, a, cfg, stream) : launch_skinny_bf16(kind, a, cfg, stream);
     return launch_mma(fdt, kind, backward, a, cfg, stream);

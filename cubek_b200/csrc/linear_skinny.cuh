@@ -7,8 +7,8 @@
 // them four at a time from every lane as if they were in the instruction's order.  Groups of 2, 4 or 8 warps share K and
 // add their sums in warp order through shared memory.
 // Codes are on their way two chunks ahead, by asynchronous copies into the warp's own ring in shared memory: whole rows of a
-// chunk at a time, and no registers, so that 24 warps fit an SM (with a ring in registers 16 did, and the latency of the
-// decoding was what 126 us for 235 MB of 4-bit codes went to).
+// chunk at a time, and no registers, so that 24 warps fit an SM (with a ring in registers 16 did: 127 us for 206 MB of
+// 4-bit codes of 7 experts, 82 now).
 #pragma once
 
 #include "linear_tiles.cuh"
@@ -48,7 +48,7 @@ template <bool WHOLE> __device__ __forceinline__ void fetch_x(uint32_t *x, const
         if (WHOLE || left <= 8 * i || left >= 8 * i + 8) {
             const uint32_t ok = left > 8 * i;
             asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %5, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\nmov.b32 %2, 0;\nmov.b32 %3, 0;\n"
-                "@p ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
+                         "@p ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];\n}"
                          : "=&r"(x[4 * i]), "=&r"(x[4 * i + 1]), "=&r"(x[4 * i + 2]), "=&r"(x[4 * i + 3])
                          : "l"(p + 8 * i), "r"(ok));
         } else {
@@ -65,12 +65,12 @@ template <int FDT> __device__ __forceinline__ void mma_m16n8k16(float *d, uint32
 {
     if constexpr (FDT == QK_BF16)
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     else
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 constexpr int SKINNY_FEATS = 16, SKINNY_ROWS = 8, SKINNY_WARPS = 8;

@@ -117,7 +117,7 @@ constexpr int WEIGHT_THREADS = 128, WEIGHT_GROUPS = 4, WEIGHT_SCALES_AHEAD = 4;
 // Shared memory of the codes and scales in flight; `scales` of a run, 0: not regular.
 __host__ __device__ constexpr int weight_bytes(int kind, int scales, int slots)
 {
-    return scales == 0 ? WEIGHT_GROUPS * (kind_bits(kind) == 8 ? StagedRuns<KIND_I8>::AHEAD : kind_bits(kind) == 4 ? StagedRuns<KIND_PACK4>::AHEAD : StagedRuns<KIND_PACK2>::AHEAD) * WEIGHT_THREADS *
+    return scales == 0 ? WEIGHT_GROUPS * (kind_bits(kind) >= 4 ? StagedRuns<KIND_I8>::AHEAD : StagedRuns<KIND_PACK2>::AHEAD) * WEIGHT_THREADS *
                              (kind_bits(kind) * 4 + 20)
                        : slots * 512 * kind_bits(kind) + WEIGHT_GROUPS * WEIGHT_SCALES_AHEAD * WEIGHT_THREADS * 4 * scales;
 }
@@ -182,8 +182,8 @@ template <int KIND, int FDT, bool BWD, int STRIDE, int SLOTS> struct WeightWarps
                 if (it < sched.total) {
 #pragma unroll
                     for (int i = 0; i < NS; ++i)
-                        copy_async4(in + i * WEIGHT_THREADS * 4, reinterpret_cast<const void *>(scale ? (scale + i * part) & ~(uintptr_t)3 : reinterpret_cast<uintptr_t>(a.codes) & ~(uintptr_t)3),
-                                    scale ? 4 : 0);
+                        copy_async4(in + i * WEIGHT_THREADS * 4,
+                                    reinterpret_cast<const void *>((scale ? scale + i * part : reinterpret_cast<uintptr_t>(a.scales)) & ~(uintptr_t)3), scale ? 4 : 0);
                     in += SCALE_SLOT;
                     if (in == ring_end) in = ring;
                     ikb += STRIDE;
@@ -204,7 +204,10 @@ template <int KIND, int FDT, bool BWD, int STRIDE, int SLOTS> struct WeightWarps
                 CodeRun<KIND> run;
                 if (!moving || a.param != QK_F32) {
                     at = scale_at(mma_tile(m, sched, t, feats_per_tile), moving ? kb : kb0);
-                    if (!moving) run.s[0] = !at ? 0u : a.param == QK_F32 ? __ldg(reinterpret_cast<const uint32_t *>(at)) : (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(at));
+                    if (!moving)
+                        run.s[0] = !at ? 0u
+                                   : a.param == QK_F32 ? __ldg(reinterpret_cast<const uint32_t *>(at))
+                                                       : (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(at));
                 }
 #pragma unroll 1
                 for (; kb < kb1; kb += STRIDE) {

@@ -16,7 +16,7 @@ from cubek_b200 import ElemType, QuantScheme, TensorHandleRef
 from cubek_b200.linear import Activation
 from cubek_b200.matmul_input import MatmulInputHandleRef
 from oracle import oracle as O
-from tests._util import NP_FLOAT, code_dtype, to_device
+from tests._util import NP_FLOAT, to_device
 
 H = TensorHandleRef.from_torch
 TORCH = {ElemType.F16: torch.float16, ElemType.BF16: torch.bfloat16}

@@ -8,10 +8,8 @@ from cubek_b200 import (ComputeClient, ElemType, QuantLevel, QuantParam, QuantSc
 from cubek_b200 import _ffi
 from cubek_b200.linear import Activation
 from cubek_b200.matmul_input import MatmulInputHandleRef
-from oracle import oracle as O
 from tests._cases import all_value_stores, scheme_id
 from tests._linear import TORCH, H, Weight, check_backward, check_forward, filled, randn
-from tests._util import to_device
 
 pytestmark = pytest.mark.gpu
 

@@ -2,10 +2,10 @@
 import pytest
 import torch
 
-from cubek_b200 import ComputeClient, ElemType, QuantLevel, QuantParam, QuantScheme, QuantStore, QuantValue, grouped_linear, linear
+from cubek_b200 import ComputeClient, QuantLevel, QuantParam, QuantScheme, QuantValue, grouped_linear, linear
 from cubek_b200.linear import Activation
-from tests._cases import all_value_stores, scheme_id
-from tests._linear import TORCH, H, Weight, check_backward, check_forward, filled, randn
+from tests._cases import scheme_id
+from tests._linear import H, Weight, check_backward, check_forward, filled, randn
 from tests.test_gpu_grouped_linear import offsets_of, run
 from tests.test_gpu_linear import BF16, F16, Q4, Q8, backward, case, forward, no_device_error, schemes
 
