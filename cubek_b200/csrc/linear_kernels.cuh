@@ -183,25 +183,12 @@ template <int FDT> __device__ __forceinline__ uint32_t scale_pair(int param, uin
     return h2_pack<FDT>(s, s);
 }
 
-// One stored word times its scale, as packed F x2 in element order.  dequant_word, but for 8-bit codes in bf16: byte b (biased
-// to 0 .. 255) in the middle of the mantissa of 2^15 is 32768 + b, and (32768 + b) s - 32896 s is exact in one
-// multiply-add (32896 = 257 * 128, so with the 8 bits of s neither product needs more than 24), which leaves a single rounding.
+// One stored word times its scale, as packed F x2 in element order: dequant_word itself, so that the weight is dequantize's to
+// the bit for every scale.  (8-bit codes in bf16 from one multiply-add, (32768 + b) s - 32896 s, is 0.5 to 2 % faster - 1 row
+// of 14336 x 4096 24.0 us, here 24.1; 16 rows 33.5 and 34.0; 4096 rows 428 and 429 - but 32896 s is no finite f32 from |s| = 2^113 on.)
 template <int FDT, int KIND> __device__ __forceinline__ void decode_word(uint32_t w, uint32_t s2, uint32_t *o)
 {
-    const float s = widen_lo<FDT>(s2);
-    if constexpr (FDT == QK_BF16 && (KIND == KIND_PACK8 || KIND == KIND_I8)) {
-        const uint32_t b = w ^ 0x80808080u;
-        const float c = -32896.0f * s;
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-            float r0, r1;
-            fma2(__uint_as_float(__byte_perm(b, 0x47000000u, 0x7404 + 16 * i)), __uint_as_float(__byte_perm(b, 0x47000000u, 0x7414 + 16 * i)), s, s,
-                 c, c, r0, r1);
-            o[i / 2] = h2_pack<FDT>(r0, r1);
-        }
-    } else {
-        dequant_word<FDT, KIND>(w, s, s2, o);
-    }
+    dequant_word<FDT, KIND>(w, widen_lo<FDT>(s2), s2, o);
 }
 
 // The run as 16 registers of packed F x2, in element order; codes past `valid` are +0 whatever the scale is.

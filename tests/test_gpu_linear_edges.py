@@ -1,0 +1,73 @@
+"""``linear`` and ``grouped_linear`` at values and sizes far from the ordinary ones."""
+import numpy as np
+import pytest
+import torch
+
+from cubek_b200 import QuantLevel, QuantParam, QuantScheme, QuantStore, QuantValue
+from tests._linear import Weight, check_backward, check_forward, randn
+from tests.test_gpu_linear import BF16, F16, backward, forward, no_device_error
+
+pytestmark = pytest.mark.gpu
+
+ROWS = [3, 40, 300]   # one for each kernel
+
+
+def q8(n, k, store, elem, scales, low=-127, high=128, param=QuantParam.F32, seed=1):
+    """A weight of random 8-bit codes in blocks of 32, one scale for each row."""
+    scheme = QuantScheme(value=QuantValue.Q8S, store=store, level=QuantLevel.block([32]), param=param)
+    codes = np.random.default_rng(seed).integers(low, high, (n, k)).astype(np.int8)
+    codes[:, :3] = [1, 0, -1] if low < 0 else 1
+    full = np.repeat(np.resize(np.asarray(scales, np.float32), n)[:, None], k // 32, 1)
+    return Weight((n, k), scheme, elem, seed, codes.view(np.uint32) if store == QuantStore.U32 else codes, np.ascontiguousarray(full))
+
+
+@pytest.mark.parametrize("store", [QuantStore.U32, QuantStore.Native])
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("k", [192, 160])
+def test_large_scales_of_8_bit_codes(rows, store, k):
+    """Scales of which no multiple of 2^15 is a finite f32: the weight is code times scale all the same, and zero for code 0."""
+    w = q8(80, k, store, BF16, [2e34, -2e34, 1.0, 1.04e34, -2.0 ** 116])
+    assert bool(w.value.isfinite().all())
+    x = (randn((rows, k), BF16, 2).float() * 0.1).bfloat16()
+    x[:, :3] = 1.0
+    y, pre = forward(w, x)
+    check_forward(y, pre, x, w.value, BF16)
+    g = (randn((rows, 80), BF16, 3).float() * 0.1).bfloat16()
+    gx, gb, gp = backward(w, g)
+    check_backward(gx, gb, gp, g, w.value, BF16)
+    no_device_error()
+
+
+@pytest.mark.parametrize("store", [QuantStore.U32, QuantStore.Native])
+@pytest.mark.parametrize("rows", ROWS)
+def test_largest_scale_of_8_bit_codes(rows, store):
+    """The largest bf16 as a scale: codes 1, 0 and -1 stay finite."""
+    w = q8(72, 64, store, BF16, [float(torch.finfo(torch.bfloat16).max)], -1, 2)
+    x = (randn((rows, 64), BF16, 2).float() * 2.0 ** -10).bfloat16()
+    y, pre = forward(w, x)
+    check_forward(y, pre, x, w.value, BF16)
+    assert bool(y.isfinite().all())
+    g = (randn((rows, 72), BF16, 3).float() * 2.0 ** -10).bfloat16()
+    gx, gb, gp = backward(w, g)
+    check_backward(gx, gb, gp, g, w.value, BF16)
+
+
+@pytest.mark.parametrize("elem,scale", [(BF16, float("inf")), (BF16, float("-inf")), (F16, float("inf")), (F16, 7e4), (F16, -1e3)])
+@pytest.mark.parametrize("rows", ROWS)
+def test_overflowing_scales_of_8_bit_codes(rows, elem, scale):
+    """Infinite scales, scales that round to an infinite f16, and products that do: infinities of the code's sign."""
+    w = q8(64, 64, QuantStore.U32, elem, [1.0], 1, 128)
+    scales, codes = w.scales.copy(), w.codes.copy()
+    scales[5] = scale
+    codes[5] = 0x7F7F7F7F if abs(scale) == 1e3 else codes[5]   # 127 * 1000 is past the largest f16
+    codes[9, 3] = 0x01000101   # a zero code: 0 * inf is no number, as dequantize has it
+    scales[9] = scale
+    v = Weight((64, 64), w.scheme, elem, 1, codes, scales)
+    x = (randn((rows, 64), elem, 2).float().abs() * 0.01 + 0.01).to(torch.float16 if elem == F16 else torch.bfloat16)
+    y, _ = forward(v, x)
+    assert bool((y[:, 5] == (float("inf") if scale > 0 else float("-inf"))).all())
+    if abs(scale) != 1e3:
+        assert bool(v.value[9].isnan().any()) and bool(y[:, 9].isnan().all())
+    keep = [i for i in range(64) if i not in (5, 9)]
+    check_forward(y[:, keep], None, x, v.value[keep], elem)
+    no_device_error()
