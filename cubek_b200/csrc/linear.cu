@@ -255,7 +255,7 @@ static int linear_backward(const QkTensor *grad_output, const QkTensor *offsets,
     const BackwardPlan plan = plan_backward(g.rows, a.n, a.experts, activation, grad_bias != nullptr, grad_pre != nullptr,
                                             !product_needs_aligned_rows(operand.rows, operand.ptr, operand.stride));
     const bool product = grad_input && g.rows > 0 && a.k > 0;
-    const bool needs = (plan.dz && product) || (grad_bias && plan.slices > 1);
+    const bool needs = plan.bytes > 0 && ((plan.dz && product) || (grad_bias && plan.slices > 1));   // nothing where there are no features
     if (needs && (!workspace || workspace_bytes < plan.bytes)) return QK_ERR_WORKSPACE;
     if (needs && reinterpret_cast<uintptr_t>(workspace) % 16) return QK_ERR_ALIGN;
 

@@ -3,8 +3,9 @@ import numpy as np
 import pytest
 import torch
 
-from cubek_b200 import QuantLevel, QuantParam, QuantScheme, QuantStore, QuantValue
-from tests._linear import Weight, check_backward, check_forward, randn
+from cubek_b200 import ComputeClient, QuantLevel, QuantParam, QuantScheme, QuantStore, QuantValue, linear
+from cubek_b200.linear import Activation
+from tests._linear import H, Weight, check_backward, check_forward, filled, randn
 from tests.test_gpu_linear import BF16, F16, backward, forward, no_device_error
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +72,17 @@ def test_overflowing_scales_of_8_bit_codes(rows, elem, scale):
     keep = [i for i in range(64) if i not in (5, 9)]
     check_forward(y[:, keep], None, x, v.value[keep], elem)
     no_device_error()
+
+
+@pytest.mark.parametrize("rows,n,k", [(4, 0, 32), (40, 0, 64), (300, 0, 64), (0, 16, 32), (4, 16, 0)])
+def test_empty_sizes_with_the_workspace_that_is_asked_for(rows, n, k):
+    """What the queries call enough is enough: nothing at all where they say zero."""
+    scheme = QuantScheme(value=QuantValue.Q8S)
+    w = Weight((n, k), scheme, BF16, 1, np.zeros((n, k // 4), np.uint32), np.ones(1, np.float32))
+    g, pre = randn((rows, n), BF16, 2), randn((rows, n), BF16, 3)
+    gx, gb = filled((rows, k), BF16), filled((n,), BF16)
+    size = linear.backward_workspace_bytes(H(g), w.handle(), BF16, activation=Activation.Gelu, bias=True)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda") if size else None
+    linear.launch_backward(ComputeClient.current(), H(g), w.handle(), H(gx), BF16, pre=H(pre), activation=Activation.Gelu, grad_bias=H(gb),
+                           workspace=None if ws is None else H(ws))
+    check_backward(gx, gb, None, g, w.value, BF16, pre, Activation.Gelu)
