@@ -24,7 +24,7 @@ static int as_matrix(const QkTensor *t, int dtype, Matrix &m)
         // one row of contiguous elements: its strides are never used
         if (m.rows != 1 || (m.cols != 1 && t->strides[t->rank - 1] != 1)) return QK_ERR_LAYOUT;
     }
-    if (m.rows >= (1ll << 31) || m.cols >= (1ll << 31)) return QK_ERR_TOO_LARGE;
+    if (m.rows > QK_LINEAR_MAX_ROWS || m.cols >= (1ll << 31)) return QK_ERR_TOO_LARGE;
     return QK_OK;
 }
 

@@ -62,7 +62,7 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
         m.tile_rows = WIDE_ROWS;
     } else if (!grouped) {
         const int tiles = (a.rows + 255) / 256;
-        m.tile_rows = round_up((a.rows + tiles - 1) / tiles, 16);
+        m.tile_rows = round_up((a.rows - 1) / tiles + 1, 16);
     } else {
         m.tile_rows = average >= 128 ? 256 : round_up(2 * average + 1, 16);
     }

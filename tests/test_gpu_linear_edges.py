@@ -86,3 +86,29 @@ def test_empty_sizes_with_the_workspace_that_is_asked_for(rows, n, k):
     linear.launch_backward(ComputeClient.current(), H(g), w.handle(), H(gx), BF16, pre=H(pre), activation=Activation.Gelu, grad_bias=H(gb),
                            workspace=None if ws is None else H(ws))
     check_backward(gx, gb, None, g, w.value, BF16, pre, Activation.Gelu)
+
+
+@pytest.fixture
+def released():
+    """Large buffers go back to the device after the test."""
+    yield
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n", [1, 8])
+def test_most_rows(n, released):
+    """2^31 - 512 rows, the most that are taken: the last ones are as right as the first."""
+    rows, k = 2 ** 31 - 512, 8
+    w = Weight((n, k), QuantScheme(value=QuantValue.Q8S, store=QuantStore.Native), BF16, 1)
+    at = torch.tensor([0, 1, 511, 512, 2 ** 30 + 5, rows - 513, rows - 2, rows - 1], device="cuda")
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    x[at] = randn((8, k), BF16, 2)
+    y = torch.full((rows, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+    linear.launch(ComputeClient.current(), H(x), w.handle(), H(y), BF16)
+    check_forward(y[at], None, x[at], w.value, BF16)
+    assert bool((y[2 ** 30 + 6:2 ** 30 + 600] == 0).all()) and bool((y[-500:-2] == 0).all())
+    if n == 8:   # rows of one element start on no 16 bytes: their gradient would copy them
+        gx = torch.full((rows, k), float("nan"), dtype=torch.bfloat16, device="cuda")
+        linear.launch_backward(ComputeClient.current(), H(y), w.handle(), H(gx), BF16)
+        check_backward(gx[at], None, None, y[at], w.value, BF16)
+    no_device_error()
