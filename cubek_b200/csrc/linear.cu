@@ -186,6 +186,10 @@ static int linear_forward(const QkTensor *input, const QkTensor *offsets, bool g
     if (bias && (rc = check_bias(bias, dtype, grouped, a.experts, a.n, false, &a.bias_stride, &a.bias_expert)) != QK_OK) return rc;
     if (grouped && (rc = check_offsets(offsets, a.experts, &a.offsets, &a.offsets64)) != QK_OK) return rc;
     if (x.rows == 0 || a.n == 0) return QK_OK;
+    a.rows = (int)x.rows;
+    a.contraction = a.k;
+    a.feats = a.n;
+    if (!product_tiles_fit(false, a)) return QK_ERR_TOO_LARGE;
     a.x = x.ptr;
     a.x_stride = x.stride;
     if (a.k > 0 && product_needs_aligned_rows(x.rows, x.ptr, x.stride)) {
@@ -195,9 +199,6 @@ static int linear_forward(const QkTensor *input, const QkTensor *offsets, bool g
         a.x_stride = (x.cols + 7) / 8 * 8;
         if ((rc = copy_rows(x, dtype, workspace, a.x_stride, stream)) != QK_OK) return rc;
     }
-    a.rows = (int)x.rows;
-    a.contraction = a.k;
-    a.feats = a.n;
     a.out = y.ptr;
     a.out_stride = y.stride;
     a.bias = bias ? bias->ptr : nullptr;
@@ -255,6 +256,10 @@ static int linear_backward(const QkTensor *grad_output, const QkTensor *offsets,
     const BackwardPlan plan = plan_backward(g.rows, a.n, a.experts, activation, grad_bias != nullptr, grad_pre != nullptr,
                                             !product_needs_aligned_rows(operand.rows, operand.ptr, operand.stride));
     const bool product = grad_input && g.rows > 0 && a.k > 0;
+    a.rows = (int)g.rows;
+    a.contraction = a.n;
+    a.feats = a.k;
+    if (product && !product_tiles_fit(true, a)) return QK_ERR_TOO_LARGE;
     const bool needs = plan.bytes > 0 && ((plan.dz && product) || (grad_bias && plan.slices > 1));   // nothing where there are no features
     if (needs && (!workspace || workspace_bytes < plan.bytes)) return QK_ERR_WORKSPACE;
     if (needs && reinterpret_cast<uintptr_t>(workspace) % 16) return QK_ERR_ALIGN;
@@ -289,9 +294,6 @@ static int linear_backward(const QkTensor *grad_output, const QkTensor *offsets,
     if (!product) return QK_OK;
     a.x = staged ? workspace : operand.ptr;
     a.x_stride = staged ? plan.dz_stride : operand.stride;
-    a.rows = (int)g.rows;
-    a.contraction = a.n;
-    a.feats = a.k;
     a.out = dx.ptr;
     a.out_stride = dx.stride;
     a.act = QK_ACT_IDENTITY;

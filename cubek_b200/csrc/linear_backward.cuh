@@ -25,6 +25,8 @@ int bias_slices(long long rows, long long n, int experts);
 cudaError_t launch_activation_backward(int fdt, const ActBackwardArgs &a, const LaunchCfg &cfg, cudaStream_t stream, int *launches);
 // Whether x [rows, ..] cannot be loaded as it lies: its rows do not start on 16 bytes.
 bool product_needs_aligned_rows(long long rows, const void *x, long long stride);
+// Whether the tiles of a product can be numbered; of `a`: rows, feats, k, experts and offsets.
+bool product_tiles_fit(bool backward, const LinearArgs &a);
 cudaError_t launch_linear_product(int fdt, int kind, bool backward, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream);
 
 }  // namespace qk

@@ -2,6 +2,7 @@
 #include "host_checks.cuh"
 #include "linear_backward.cuh"
 #include "linear_narrow.cuh"
+#include "linear_skinny.cuh"
 #include "linear_wide.cuh"
 
 namespace qk {
@@ -69,7 +70,6 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     row_tiles = (a.rows + m.tile_rows - 1) / m.tile_rows;
     if (grouped) row_tiles += a.experts < a.rows ? a.experts : a.rows;   // at most
     const long long tiles = row_tiles * m.feat_tiles;
-    if (tiles >= (1ll << 31)) return cudaErrorInvalidConfiguration;
     if (!wide)
         while (m.split < 8 && tiles * m.split * 2 <= cfg.sm_count && m.kblocks / (m.split * 2) >= 4) m.split *= 2;
     mma_steps(m, backward, wide ? WEIGHT_GROUPS : 2);
@@ -119,11 +119,21 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     return launches[wide][backward][fdt == QK_BF16](kind, xmap, wmap, m, grid, smem, cfg, stream);
 }
 
+// A handful of rows (of an expert, on average): 14336 x 4096 q8 with 8 rows 22 us, with 9 on the tiles of the tensor
+// cores 31; of each of 8 experts, q4, 148 and 202 us, q8 both 195.
+static bool handful(bool backward, const LinearArgs &a) { return !backward && a.k > 0 && a.rows <= SKINNY_ROWS * a.experts; }
+
+// Tiles are numbered by 32-bit integers, and a CTA steps past the last one by less than 2^20.
+bool product_tiles_fit(bool backward, const LinearArgs &a)
+{
+    const bool few = handful(backward, a);
+    const long long partial = !a.offsets ? 0 : a.experts < a.rows ? a.experts : a.rows;
+    return (a.rows / (few ? SKINNY_ROWS : 16) + 1 + partial) * (a.feats / (few ? SKINNY_FEATS : 128) + 1ll) < (1ll << 31) - (1 << 20);
+}
+
 cudaError_t launch_linear_product(int fdt, int kind, bool backward, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
 {
-    // A handful of rows (of an expert, on average): 14336 x 4096 q8 with 8 rows 22 us, with 9 on the tiles of the tensor
-    // cores 31; of each of 8 experts, q4, 148 and 202 us, q8 both 195.
-    if (!backward && a.k > 0 && a.rows <= 8 * a.experts)
+    if (handful(backward, a))
         return fdt == QK_F16 ? launch_skinny_f16(kind, a, cfg, stream) : launch_skinny_bf16(kind, a, cfg, stream);
     return launch_mma(fdt, kind, backward, a, cfg, stream);
 }

@@ -322,7 +322,6 @@ static cudaError_t launch_skinny_rows(const LinearArgs &a, long long row_tiles, 
     m.feat_tiles = (a.feats + SKINNY_FEATS * R - 1) / (SKINNY_FEATS * R);
     m.by_feat_tiles = make_fastdiv((unsigned)m.feat_tiles);
     const long long tiles = row_tiles * m.feat_tiles, resident = cfg.sm_count * (NS < 4 ? 3 : 2);
-    if (tiles >= (1ll << 31)) return cudaErrorInvalidConfiguration;
     m.split = split;
     const size_t smem = skinny_bytes(kind_bits(KIND), R, NS) + (a.offsets ? (3 * a.experts + 1) * 4 : 0);
     int dev = 0;
