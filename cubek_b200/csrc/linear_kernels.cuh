@@ -47,13 +47,14 @@ struct LinearArgs {
     int *error_flag;
 };
 
-// Rows of expert e.  Offsets are clamped to the tensor, so that wrong ones give wrong rows, not wrong addresses.
-__device__ __forceinline__ void expert_rows(const LinearArgs &a, int e, int &lo, int &hi)
+// Rows of expert e; returns whether its offsets descend.  They are clamped to the tensor, so that wrong ones give wrong rows,
+// not wrong addresses.
+__device__ __forceinline__ bool expert_rows(const LinearArgs &a, int e, int &lo, int &hi)
 {
     if (a.offsets == nullptr) {
         lo = 0;
         hi = a.rows;
-        return;
+        return false;
     }
     long long l, h;
     if (a.offsets64) {
@@ -63,10 +64,12 @@ __device__ __forceinline__ void expert_rows(const LinearArgs &a, int e, int &lo,
         l = static_cast<const int *>(a.offsets)[e];
         h = static_cast<const int *>(a.offsets)[e + 1];
     }
+    const bool descend = h < l;
     l = l < 0 ? 0 : l > a.rows ? a.rows : l;
     h = h < l ? l : h > a.rows ? a.rows : h;
     lo = (int)l;
     hi = (int)h;
+    return descend;
 }
 
 // ---- activations, in f32 --------------------------------------------------------------------------

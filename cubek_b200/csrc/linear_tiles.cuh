@@ -76,13 +76,26 @@ __device__ __forceinline__ MmaSchedule mma_schedule(const LinearMmaArgs &m, int 
     }
     int *prefix = table, *lo = table + a.experts + 1, *hi = lo + a.experts;
     const int lane = threadIdx.x % 32;
+    int descend = 0;
     for (int e = threadIdx.x; e < a.experts; e += threads) {
         int l, h;
-        expert_rows(a, e, l, h);
+        descend |= expert_rows(a, e, l, h);
         lo[e] = l;
         hi[e] = h;
     }
-    __syncthreads();
+    // Only offsets that descend somewhere can name a row twice.  It goes to the first expert: two would write it in any order,
+    // and the tiles would be more than were counted before the launch.
+    if (__syncthreads_or(descend)) {
+        if (threadIdx.x == 0) {
+            int taken = 0;
+            for (int e = 0; e < a.experts; ++e) {
+                lo[e] = max(lo[e], taken);
+                hi[e] = max(hi[e], lo[e]);
+                if (hi[e] > lo[e]) taken = hi[e];
+            }
+        }
+        __syncthreads();
+    }
     if (threadIdx.x < 32) {   // running sum of the experts' tiles of rows
         int sum = 0;
         for (int e0 = 0; e0 < a.experts; e0 += 32) {

@@ -321,8 +321,8 @@ int qk_linear(const QkTensor *input, const QkTensor *values, const QkTensor *par
  * The same for E <= QK_LINEAR_MAX_EXPERTS experts: values [E, N, K / num_quants], params with a leading dim per block
  * (one scale in all per tensor), bias [E, N].  The rows of x are sorted by expert: rows offsets[e] .. offsets[e + 1]
  * use W[e] and bias[e].  `offsets` is a device array of E + 1 int32 or int64 in ascending order, 0 <= offsets <= rows
- * (others are clamped); an expert may have no rows.  Rows outside [offsets[0], offsets[E]) are left as they were in
- * every output.
+ * (others are clamped; a row that descending ones name twice is the first expert's, and counts in any grad_bias); an expert
+ * may have no rows.  Rows outside [offsets[0], offsets[E]) are left as they were in every output.
  */
 #define QK_LINEAR_MAX_EXPERTS 1024
 int qk_grouped_linear(const QkTensor *input, const QkTensor *offsets, const QkTensor *values, const QkTensor *params, const QkScheme *scheme,

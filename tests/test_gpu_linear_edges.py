@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from cubek_b200 import ComputeClient, QuantLevel, QuantParam, QuantScheme, QuantStore, QuantValue, linear
+from cubek_b200 import ComputeClient, QuantLevel, QuantParam, QuantScheme, QuantStore, QuantValue, grouped_linear, linear
 from cubek_b200.linear import Activation
 from tests._linear import H, Weight, check_backward, check_forward, filled, randn
 from tests.test_gpu_linear import BF16, F16, backward, forward, no_device_error
@@ -111,4 +111,20 @@ def test_most_rows(n, released):
         gx = torch.full((rows, k), float("nan"), dtype=torch.bfloat16, device="cuda")
         linear.launch_backward(ComputeClient.current(), H(y), w.handle(), H(gx), BF16)
         check_backward(gx[at], None, None, y[at], w.value, BF16)
+    no_device_error()
+
+
+@pytest.mark.parametrize("rows", [20, 60, 1000])
+def test_offsets_that_overlap(rows):
+    """Descending offsets that name rows twice: the first expert has them, whatever the timing."""
+    w = Weight((5, 72, 96), QuantScheme(value=QuantValue.Q4S, level=QuantLevel.block([32])), BF16, 1)
+    x = (randn((rows, 96), BF16, 2).float() * 0.2).bfloat16()
+    half = rows // 2
+    off = torch.tensor([0, half, 0, half + 5, 3, rows], dtype=torch.int32, device="cuda")
+    owner = [(0, 0, half), (2, half, half + 5), (4, half + 5, rows)]   # expert, its rows
+    for _ in range(3):
+        y = filled((rows, 72), BF16)
+        grouped_linear.launch(ComputeClient.current(), H(x), H(off), w.handle(), H(y), BF16)
+        for e, lo, hi in owner:
+            check_forward(y[lo:hi], None, x[lo:hi], w.value[e], BF16)
     no_device_error()
