@@ -127,10 +127,11 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1) linear_narrow_kernel(const 
     const uint32_t tmem = tmem_slot;
 
     // Every wait is bounded: a thread that gives up says so to the others of its CTA and to the host, and from then on
-    // waits for nothing and starts nothing.
+    // waits for nothing and starts nothing.  A wait for a whole sum may take longer by its steps (1.5 us each at most, for rows
+    // of codes that start on no word, on a GPU of its own).
     bool dead = false;
-    const auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (!dead && !mbar_wait(bar, parity, &gave_up)) {
+    const auto wait = [&](uint32_t bar, uint32_t parity, int sum_steps = 0) {
+        if (!dead && !mbar_wait(bar, parity, &gave_up, sum_steps)) {
             dead = true;
             *(volatile int *)&gave_up = 1;
             atomicExch(a.error_flag, 1);
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(NARROW_THREADS, 1) linear_narrow_kernel(const 
             const uint32_t from = tmem + ((uint32_t)warp << 21) + buf * m.tile_rows;   // lane 32 * warp
             const bool sums = kb0 < kb1;
             if (sums) {
-                wait(acc_full(buf), buf_phase);
+                wait(acc_full(buf), buf_phase, kb1 - kb0);
                 dead = __any_sync(0xffffffffu, dead);
                 tc_fence_after();
             }

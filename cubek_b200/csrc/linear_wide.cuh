@@ -127,10 +127,11 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) linear_wide_kernel(const __gr
     const uint32_t tmem = tmem_slot;
 
     // Every wait is bounded: a thread that gives up says so to the others of its CTA and to the host, and from then on
-    // waits for nothing and starts nothing.
+    // waits for nothing and starts nothing.  A wait for a whole sum may take longer by its steps (1.5 us each at most, for rows
+    // of codes that start on no word, on a GPU of its own).
     bool dead = false;
-    const auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (!dead && !mbar_wait(bar, parity, &gave_up)) {
+    const auto wait = [&](uint32_t bar, uint32_t parity, int sum_steps = 0) {
+        if (!dead && !mbar_wait(bar, parity, &gave_up, sum_steps)) {
             dead = true;
             *(volatile int *)&gave_up = 1;
             atomicExch(a.error_flag, 1);
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, 1) linear_wide_kernel(const __gr
             const MmaTile tile = mma_tile(m, sched, t, WIDE_FEATS);
             bias_tile[buf][threadIdx.x] = load_bias<FDT>(a, tile.e, tile.f0 + (int)threadIdx.x);
             asm volatile("bar.sync 2, 128;" ::: "memory");   // the other buffer's readers have passed here once since
-            wait(acc_full(buf), buf_phase);
+            wait(acc_full(buf), buf_phase, steps);
             dead = __any_sync(0xffffffffu, dead);
             tc_fence_after();
             const uint32_t from = tmem + ((uint32_t)warp << 21) + buf * 256;

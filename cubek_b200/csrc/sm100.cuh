@@ -36,23 +36,25 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity)
     return ok != 0;
 }
 
-// Waits at most two seconds; `stop`: also ends when another thread of the CTA has given up.
-static __device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, const int *stop)
+// Waits at most two seconds, and 16 us for each of the `steps` that the awaited work takes; `stop`: also ends when another
+// thread of the CTA has given up.
+static __device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, const int *stop, int steps)
 {
+    const unsigned long long limit = 2000000000ull + 16000ull * (unsigned)steps;
     unsigned long long start, now;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
     for (int i = 0;; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 63) == 63) {
             asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-            if (now - start > 2000000000ull || (stop && *(const volatile int *)stop)) return false;
+            if (now - start > limit || (stop && *(const volatile int *)stop)) return false;
         }
     }
 }
 
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const int *stop)
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const int *stop, int steps = 0)
 {
-    return mbar_try_wait(bar, parity) || mbar_wait_long(bar, parity, stop);
+    return mbar_try_wait(bar, parity) || mbar_wait_long(bar, parity, stop, steps);
 }
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one()

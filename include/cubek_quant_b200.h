@@ -304,9 +304,9 @@ int qk_into_contiguous_packed(const QkTensor *input, const QkTensor *output, con
  *   output    y [.., N], typed as x; overlaps no input but `residual`
  *   pre       [.., N], receives x W^T + bias (rounded), which the gradient of the activation needs; NULL: not kept
  * A column-major operand (packed along N) is QK_ERR_LAYOUT: qk_into_contiguous_packed makes it row-major.  N and K are
- * below QK_LINEAR_MAX_EXTENT (a sum of that length takes the tensor cores half a second, and their waits end after
- * two); there are QK_LINEAR_MAX_ROWS rows at most (rounded up to a tile they are 32-bit integers).  As with the other entry
- * points, make the first call on a device before any stream capture.
+ * below QK_LINEAR_MAX_EXTENT (a sum of that length takes up to one and a half seconds, a wait for it ends after 18); there are
+ * QK_LINEAR_MAX_ROWS rows at most (rounded up to a tile they are 32-bit integers).  As with the other entry points, make the
+ * first call on a device before any stream capture.
  */
 #define QK_LINEAR_MAX_EXTENT (1ll << 26)
 #define QK_LINEAR_MAX_ROWS ((1ll << 31) - 512)

@@ -5,6 +5,7 @@ import torch
 
 from cubek_b200 import ComputeClient, QuantLevel, QuantParam, QuantScheme, QuantStore, QuantValue, grouped_linear, linear
 from cubek_b200.linear import Activation
+from cubek_b200.matmul_input import MatmulInputHandleRef
 from tests._linear import H, Weight, check_backward, check_forward, filled, randn
 from tests.test_gpu_linear import BF16, F16, backward, forward, no_device_error
 
@@ -128,3 +129,20 @@ def test_offsets_that_overlap(rows):
         for e, lo, hi in owner:
             check_forward(y[lo:hi], None, x[lo:hi], w.value[e], BF16)
     no_device_error()
+
+
+def test_a_sum_of_the_longest_extent(released):
+    """2^26 - 1 terms on the path of unaligned rows of codes, where a step takes longest: no wait may end before the sum does."""
+    rows, n, k = 160, 16, (1 << 26) - 1
+    scheme = QuantScheme(value=QuantValue.Q8S, store=QuantStore.Native)
+    codes = torch.zeros(n, k, dtype=torch.int8, device="cuda")
+    scale = torch.full((1,), 0.5, device="cuda")
+    x = torch.zeros(rows, k + 1, dtype=torch.bfloat16, device="cuda")[:, :k]
+    at = torch.tensor([0, 1, 63, 64, (1 << 25) + 7, k - 1], device="cuda")
+    codes[:, at] = torch.randint(-127, 128, (n, 6), device="cuda", dtype=torch.int8)
+    x[:, at] = randn((rows, 6), BF16, 3)
+    y = filled((rows, n), BF16)
+    linear.launch(ComputeClient.current(), H(x), MatmulInputHandleRef.quantized(H(codes), H(scale), (n, k), scheme), H(y), BF16)
+    torch.cuda.synchronize()
+    no_device_error()
+    check_forward(y, None, x[:, at], codes[:, at].double() * 0.5, BF16)
