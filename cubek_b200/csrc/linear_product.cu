@@ -53,25 +53,33 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     m.kblocks = (a.contraction + 63) / 64;
     m.feat_tiles = (a.feats + 127) / 128;
     m.by_feat_tiles = make_fastdiv((unsigned)m.feat_tiles);
+    const long long partial = !grouped ? 0 : a.experts < a.rows ? a.experts : a.rows;   // tiles of rows that experts may add
+    const auto tiles_of = [&](int tile_rows) { return ((a.rows - 1) / tile_rows + 1 + partial) * m.feat_tiles; };
+    if (!grouped) m.tile_rows = round_up((a.rows - 1) / ((a.rows + 255) / 256) + 1, 16);
+    else m.tile_rows = average >= 128 ? 256 : round_up(2 * average + 1, 16);
+    long long tiles = tiles_of(m.tile_rows);
     m.split = 1;
+    while (m.split < 8 && tiles * m.split * 2 <= cfg.sm_count && m.kblocks / (m.split * 2) >= 4) m.split *= 2;
     // Pairs of CTAs from 160 rows (of an expert, on average): 8 experts 14336 x 4096 q4 with 128 and 159 rows on the other kernel
     // 264 and 270 us, 128 and 192 rows on pairs 277 and 293; one 4096 x 4096 with 159 rows 27, on pairs 27.  Pairs store a row's
     // features from one lane, which rows that start on no 16 bytes would turn into single elements all over memory.
-    const bool wide = average >= 160 && m.kblocks > 0 && a.wide;
-    long long row_tiles;
+    // Pairs do not split the contraction, so few tiles of a long one are left to the other kernel: a step of it takes twice as
+    // long (0.7 to 0.85 us, of a pair 0.30 to 0.37), and the exchange of a split sum as long as some 64.  us of the other
+    // kernel and of pairs, a call at a time: 1024 x 14336 with 160 rows 39 and 76, 512 rows 77 and 92, 1024 rows 63 and 94,
+    // 2048 rows 100 and 98; 4096 x 14336 with 160 rows 53 and 78, 384 rows 92 and 94, 768 rows 133 and 98; 512 x 4096 with
+    // 512 rows 35 and 37, 1024 x 4096 with 512 rows 55 and 37, 4096 x 4096 with 256 rows 41 and 31.
+    const long long tiles_wide = tiles_of(WIDE_ROWS);
+    const auto rounds = [&](long long count, int members) {
+        const int at_once = cfg.sm_count / members;
+        return (count + at_once - 1) / at_once;
+    };
+    const long long steps = rounds(tiles, m.split) * ((m.kblocks + m.split - 1) / m.split), steps_wide = rounds(tiles_wide, 2) * m.kblocks;
+    const bool wide = average >= 160 && m.kblocks > 0 && a.wide && steps_wide <= 2 * steps + 64;
     if (wide) {
         m.tile_rows = WIDE_ROWS;
-    } else if (!grouped) {
-        const int tiles = (a.rows + 255) / 256;
-        m.tile_rows = round_up((a.rows - 1) / tiles + 1, 16);
-    } else {
-        m.tile_rows = average >= 128 ? 256 : round_up(2 * average + 1, 16);
+        m.split = 1;
+        tiles = tiles_wide;
     }
-    row_tiles = (a.rows + m.tile_rows - 1) / m.tile_rows;
-    if (grouped) row_tiles += a.experts < a.rows ? a.experts : a.rows;   // at most
-    const long long tiles = row_tiles * m.feat_tiles;
-    if (!wide)
-        while (m.split < 8 && tiles * m.split * 2 <= cfg.sm_count && m.kblocks / (m.split * 2) >= 4) m.split *= 2;
     mma_steps(m, backward, wide ? WEIGHT_GROUPS : 2);
     const int stage_bytes = wide ? WIDE_STAGE : A_BYTES + m.tile_rows * 128, table = grouped ? (3 * a.experts + 1) * 4 : 0;
     const int runs = weight_bytes(kind, m.regular ? a.run_scales : 0, wide ? WIDE_SLOTS : NARROW_SLOTS);

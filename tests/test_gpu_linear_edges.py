@@ -146,3 +146,34 @@ def test_a_sum_of_the_longest_extent(released):
     torch.cuda.synchronize()
     no_device_error()
     check_forward(y, None, x[:, at], codes[:, at].double() * 0.5, BF16)
+
+
+@pytest.mark.parametrize("rows", [160, 333, 700])
+@pytest.mark.parametrize("n", [72, 264])
+def test_few_tiles_and_a_long_sum(rows, n):
+    """Many rows of few features: tiles that fill little of the machine, whose contraction is split instead."""
+    k = 16384
+    w = Weight((n, k), QuantScheme(value=QuantValue.Q4S, level=QuantLevel.block([32])), BF16, 1)
+    x = (randn((rows, k), BF16, 2).float() * 0.01).bfloat16()
+    bias = randn((n,), BF16, 3)
+    y, pre = forward(w, x, bias, act=Activation.Silu)
+    check_forward(y, pre, x, w.value, BF16, bias, act=Activation.Silu)
+    v = Weight((k, n), QuantScheme(value=QuantValue.Q4S, level=QuantLevel.block([8])), BF16, 1)
+    g = (randn((rows, k), BF16, 4).float() * 0.01).bfloat16()
+    gx, gb, gp = backward(v, g)
+    check_backward(gx, gb, gp, g, v.value, BF16)
+    no_device_error()
+
+
+def test_few_tiles_of_experts_and_a_long_sum():
+    w = Weight((3, 72, 16384), QuantScheme(value=QuantValue.Q4S, level=QuantLevel.block([32])), BF16, 1)
+    counts = [200, 0, 300]
+    x = (randn((500, 16384), BF16, 2).float() * 0.01).bfloat16()
+    off = torch.tensor([0, 200, 200, 500], dtype=torch.int32, device="cuda")
+    y = filled((500, 72), BF16)
+    grouped_linear.launch(ComputeClient.current(), H(x), H(off), w.handle(), H(y), BF16)
+    lo = 0
+    for e, c in enumerate(counts):
+        check_forward(y[lo:lo + c], None, x[lo:lo + c], w.value[e], BF16)
+        lo += c
+    no_device_error()
