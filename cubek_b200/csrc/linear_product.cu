@@ -44,6 +44,14 @@ static EncodeTiled encode_tiled()
 
 static int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
+// Clusters of 1, 2, 4 or 8 CTAs that run at once with a CTA per SM.  One of 4 or 8 has to lie in one group of SMs: of the 148 SMs
+// 132 and 120 take part (cudaOccupancyMaxActiveClusters), and a 16th cluster of 8 waits for another to end: 16 rows of
+// 2048 x 4096, 16 tiles, 24.0 us on clusters of 8, 16.5 on clusters of 4; 34 tiles, 30.2 on clusters of 4, 23.5 on those of 2.
+static int resident_clusters(int members, const LaunchCfg &cfg)
+{
+    return members <= 2 ? cfg.sm_count / members : members == 4 ? cfg.sm_count * 33 / 148 : cfg.sm_count * 15 / 148;
+}
+
 static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs &a, const LaunchCfg &cfg, cudaStream_t stream)
 {
     LinearMmaArgs m = {};
@@ -59,7 +67,7 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     else m.tile_rows = average >= 128 ? 256 : round_up(2 * average + 1, 16);
     long long tiles = tiles_of(m.tile_rows);
     m.split = 1;
-    while (m.split < 8 && tiles * m.split * 2 <= cfg.sm_count && m.kblocks / (m.split * 2) >= 4) m.split *= 2;
+    while (m.split < 8 && tiles <= resident_clusters(m.split * 2, cfg) && m.kblocks / (m.split * 2) >= 4) m.split *= 2;
     // Pairs of CTAs from 160 rows (of an expert, on average): 8 experts 14336 x 4096 q4 with 128 and 159 rows on the other kernel
     // 264 and 270 us, 128 and 192 rows on pairs 277 and 293; one 4096 x 4096 with 159 rows 27, on pairs 27.  Pairs store a row's
     // features from one lane, which rows that start on no 16 bytes would turn into single elements all over memory.
@@ -70,7 +78,7 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     // 512 rows 35 and 37, 1024 x 4096 with 512 rows 55 and 37, 4096 x 4096 with 256 rows 41 and 31.
     const long long tiles_wide = tiles_of(WIDE_ROWS);
     const auto rounds = [&](long long count, int members) {
-        const int at_once = cfg.sm_count / members;
+        const int at_once = resident_clusters(members, cfg);
         return (count + at_once - 1) / at_once;
     };
     const long long steps = rounds(tiles, m.split) * ((m.kblocks + m.split - 1) / m.split), steps_wide = rounds(tiles_wide, 2) * m.kblocks;
