@@ -119,7 +119,7 @@ __device__ __forceinline__ float activation_slope(int act, float z)
     }
     case QK_ACT_GELU_TANH: {
         const float s = sigmoid_f32(1.59576912f * (z + 0.044715f * z * z * z));
-        return s + z * s * (1.0f - s) * 1.59576912f * (1.0f + 0.134145f * z * z);
+        return s + z * s * (1.0f - s) * 1.59576912f * (1.0f + 0.134145f * fminf(z * z, 1e30f));   // s (1 - s) is zero long before: no 0 inf
     }
     case QK_ACT_SILU: {
         const float s = sigmoid_f32(z);

@@ -177,3 +177,20 @@ def test_few_tiles_of_experts_and_a_long_sum():
         check_forward(y[lo:lo + c], None, x[lo:lo + c], w.value[e], BF16)
         lo += c
     no_device_error()
+
+
+@pytest.mark.parametrize("act", [Activation.Gelu, Activation.GeluTanh, Activation.Silu])
+def test_slopes_at_far_values(act):
+    """Far from zero the slope is one or zero, also where squares and cubes of the pre-activation are no finite f32."""
+    w = Weight((64, 64), QuantScheme(value=QuantValue.Q8S), BF16, 1)
+    far = torch.tensor([1e3, 1e10, 1e13, 1.7e19, 2e19, 1e20, 1e30, 3e38], device="cuda").bfloat16()
+    pre = torch.cat([far, -far]).repeat(4).expand(20, 64).contiguous()
+    g = randn((20, 64), BF16, 2)
+    _, gb, gp = backward(w, g, pre, act)
+    assert torch.equal(gp, torch.where(pre > 0, g, torch.zeros_like(g)))
+    want = torch.where(pre > 0, g, torch.zeros_like(g)).double()
+    assert bool(((gb.double() - want.sum(0)).abs() <= 36 * 2.0 ** -23 * want.abs().sum(0) * 1.01 + 2.0 ** -8 * want.sum(0).abs()).all())
+    y = torch.zeros(20, 64, dtype=torch.bfloat16, device="cuda")
+    bias = pre[0].contiguous()
+    out, _ = forward(w, y, bias, act=act)
+    assert torch.equal(out, torch.where(pre > 0, pre, torch.zeros_like(pre)))
