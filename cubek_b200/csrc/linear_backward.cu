@@ -8,12 +8,13 @@
 
 namespace qk {
 
-// g *= act'(z) for N values, chosen outside the loop.
+// g *= act'(z) for N values, chosen outside the loop.  Where ReLU is flat it passes zero whatever g is: infinities and NaN of an
+// overflown loss stay out.
 template <int N> __device__ __forceinline__ void slope_all(int act, float *g, const float *z)
 {
     if (act == QK_ACT_RELU) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) g[i] *= activation_slope(QK_ACT_RELU, z[i]);
+        for (int i = 0; i < N; ++i) g[i] = z[i] > 0.0f ? g[i] : 0.0f;
     } else if (act == QK_ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < N; ++i) g[i] *= activation_slope(QK_ACT_SILU, z[i]);

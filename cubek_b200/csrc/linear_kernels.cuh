@@ -111,7 +111,6 @@ __device__ __forceinline__ float activate(int act, float z)
 __device__ __forceinline__ float activation_slope(int act, float z)
 {
     switch (act) {
-    case QK_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
     case QK_ACT_GELU: {
         float bell;
         const float cdf = normal_cdf(z, bell);

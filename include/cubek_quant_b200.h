@@ -333,8 +333,9 @@ int qk_grouped_linear(const QkTensor *input, const QkTensor *offsets, const QkTe
  * Gradients.  With g = dL/dy:  dz = g act'(pre),  grad_input = dz W,  grad_bias = sum of dz over the rows (of the expert),
  * and the gradient of the residual is g itself.  Codes are integers and scales constants: they have no gradient here;
  * `grad_pre` receives dz (rounded) for callers that train weights behind the codes.
- * dz is rounded to the type of x before the product (it is an operand of the tensor cores); grad_bias sums the
- * unrounded ones in f32 and is rounded once.
+ * The slope is taken at `pre` as it is stored, rounded to the type of x; ReLU's is zero at 0, and where it is zero dz is too,
+ * whatever g holds.  dz is rounded to the type of x before the product (it is an operand of the tensor cores); grad_bias sums
+ * the unrounded ones in f32 and is rounded once.
  *   pre        what the forward pass left in `pre`; may be NULL with QK_ACT_IDENTITY
  *   grad_input, grad_bias, grad_pre   each may be NULL: not computed.  grad_bias of an expert without rows is zero.
  */

@@ -194,3 +194,17 @@ def test_slopes_at_far_values(act):
     bias = pre[0].contiguous()
     out, _ = forward(w, y, bias, act=act)
     assert torch.equal(out, torch.where(pre > 0, pre, torch.zeros_like(pre)))
+
+
+@pytest.mark.parametrize("n", [64, 37])
+def test_relu_passes_nothing_where_it_is_flat(n):
+    """An infinite or undefined incoming gradient (an overflown loss scale) stays out of the places where ReLU is flat."""
+    w = Weight((n, 64), QuantScheme(value=QuantValue.Q8S), F16, 1)
+    pre, g = randn((50, n), F16, 2), randn((50, n), F16, 3)
+    flat = ~(pre > 0)
+    flat[:, 0], pre[:, 0] = True, 0.0
+    g = torch.where(flat & (torch.arange(n, device="cuda") % 3 == 0), torch.full_like(g, float("inf")), g)
+    g = torch.where(flat & (torch.arange(n, device="cuda") % 3 == 1), torch.full_like(g, float("nan")), g)
+    gx, gb, gp = backward(w, g, pre, Activation.Relu)
+    clean = torch.where(flat, torch.zeros_like(g), g)
+    check_backward(gx, gb, gp, clean, w.value, F16, pre, Activation.Relu)
