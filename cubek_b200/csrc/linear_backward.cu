@@ -118,7 +118,7 @@ template <int FDT> __global__ void __launch_bounds__(256) bias_gradient_kernel(c
     static_cast<F *>(a.grad_bias)[e * a.grad_bias_expert + c * a.grad_bias_stride] = (F)s;
 }
 
-// Three CTAs for each of 148 SMs, and no slice below 32 rows of an evenly filled expert.
+// Six CTAs of strips of 256 columns for each of 148 SMs, and no slice below 32 rows of an evenly filled expert.
 int bias_slices(long long rows, long long n, int experts)
 {
     const long long strips = (n + 255) / 256;

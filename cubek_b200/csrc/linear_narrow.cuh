@@ -19,6 +19,9 @@ constexpr int NARROW_FEATS = 128, NARROW_SLOTS = 12;
 constexpr int NARROW_WEIGHT_FIRST = 224;   // warps 0-3 epilogue, 4 loads x, 5 products, 6 loads codes, then weight
 constexpr int NARROW_THREADS = NARROW_WEIGHT_FIRST + WEIGHT_GROUPS * WEIGHT_THREADS;
 constexpr int A_BYTES = 128 * 64 * 2;
+// three stages at least: the exchange of a split contraction needs 512 bytes a row
+static_assert(3 * (A_BYTES + 256 * 128) <= MMA_SMEM_LIMIT - MMA_SMEM_OTHER - weight_bytes_most(NARROW_SLOTS), "the stages do not fit");
+static_assert(256 * 512 <= 3 * (A_BYTES + 256 * 128) && 16 * 512 <= 3 * (A_BYTES + 16 * 128), "the exchange does not fit");
 
 // 16 sums of one feature per lane, rows row .. row + 15 of which `valid` exist.
 template <int FDT>

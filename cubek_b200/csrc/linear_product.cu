@@ -91,7 +91,6 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     mma_steps(m, backward, wide ? WEIGHT_GROUPS : 2);
     const int stage_bytes = wide ? WIDE_STAGE : A_BYTES + m.tile_rows * 128, table = grouped ? (3 * a.experts + 1) * 4 : 0;
     const int runs = weight_bytes(kind, m.regular ? a.run_scales : 0, wide ? WIDE_SLOTS : NARROW_SLOTS);
-    // three stages at least (at most 48 KiB each, 64 of runs, 12 of table): the exchange of a split contraction needs 512 bytes a row
     m.stages = (MMA_SMEM_LIMIT - 1024 - table - runs) / stage_bytes;
     if (m.stages > MMA_MAX_STAGES) m.stages = MMA_MAX_STAGES;
     if (wide) m.stages = WIDE_STAGES;

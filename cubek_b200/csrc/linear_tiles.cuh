@@ -134,6 +134,16 @@ __host__ __device__ constexpr int weight_bytes(int kind, int scales, int slots)
                              (kind_bits(kind) * 4 + 20)
                        : slots * 512 * kind_bits(kind) + WEIGHT_GROUPS * WEIGHT_SCALES_AHEAD * WEIGHT_THREADS * 4 * scales;
 }
+// Of every kind of code: 8-bit ones take most either way, or 2-bit ones, whose irregular runs are copied a step further ahead.
+__host__ __device__ constexpr int weight_bytes_most(int slots)
+{
+    int most = 0;
+    for (const int kind : {KIND_I8, KIND_PACK4, KIND_PACK2})
+        for (const int scales : {0, 1, 2}) most = weight_bytes(kind, scales, slots) > most ? weight_bytes(kind, scales, slots) : most;
+    return most;
+}
+// Shared memory beside stages and runs: up to a boundary of 1 KiB, and the table of the most experts.
+constexpr int MMA_SMEM_OTHER = 1024 + (3 * QK_LINEAR_MAX_EXPERTS + 1) * 4;
 
 // STRIDE: steps from one of a group's to its next.  SLOTS: tiles of codes in flight to the CTA; a group takes every fourth.
 template <int KIND, int FDT, bool BWD, int STRIDE, int SLOTS> struct WeightWarps {

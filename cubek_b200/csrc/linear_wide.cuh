@@ -17,7 +17,8 @@ constexpr int WIDE_ROWS = 512, WIDE_FEATS = 128;          // tile of a pair
 constexpr int WIDE_FIRST = 224;                           // warps 0-3 epilogue, 4 loads x, 5 products, 6 loads codes, then weight
 constexpr int WIDE_THREADS = WIDE_FIRST + WEIGHT_GROUPS * WEIGHT_THREADS;
 constexpr int WIDE_X_BYTES = 128 * 64 * 2, WIDE_STAGE = 2 * WIDE_X_BYTES + 64 * 64 * 2;
-constexpr int WIDE_SLOTS = 8, WIDE_STAGES = 4;   // 160 KiB, and at most 48 of runs and 12 of table
+constexpr int WIDE_SLOTS = 8, WIDE_STAGES = 4;   // 160 KiB, and at most 52 of runs and 12 of table
+static_assert(WIDE_STAGES * WIDE_STAGE <= MMA_SMEM_LIMIT - MMA_SMEM_OTHER - weight_bytes_most(WIDE_SLOTS), "the stages do not fit");
 
 // 16 sums of neighbouring features f .. f + 15 of one row.
 template <int FDT> __device__ __forceinline__ void wide_store16(const LinearArgs &a, float *v, long long row, int f, const float *bias)

@@ -208,3 +208,22 @@ def test_relu_passes_nothing_where_it_is_flat(n):
     gx, gb, gp = backward(w, g, pre, Activation.Relu)
     clean = torch.where(flat, torch.zeros_like(g), g)
     check_backward(gx, gb, gp, clean, w.value, F16, pre, Activation.Relu)
+
+
+def test_most_experts_with_unaligned_codes():
+    """1024 experts on the tiles for many rows, with rows of 8-bit codes that start anywhere: the most shared memory a call takes."""
+    e, n, k = 1024, 16, 33
+    scheme = QuantScheme(value=QuantValue.Q8S, store=QuantStore.Native, level=QuantLevel.block([8]))
+    w = Weight((e, n, k), scheme, BF16, 1)
+    counts = torch.tensor([(i * 37) % 321 for i in range(e)])
+    rows = int(counts.sum())
+    off = torch.cat([counts.new_zeros(1), counts.cumsum(0)]).to(torch.int32).cuda()
+    x = randn((rows, 40), BF16, 2)[:, :k]
+    y = filled((rows, n), BF16)
+    grouped_linear.launch(ComputeClient.current(), H(x), H(off), w.handle(), H(y), BF16)
+    owner = torch.repeat_interleave(torch.arange(e), counts).cuda()
+    x64 = x.double()[:, :, None]
+    want = torch.bmm(w.value[owner], x64)[:, :, 0]
+    tol = (k + 16) * 2.0 ** -23 * torch.bmm(w.value[owner].abs(), x64.abs())[:, :, 0]
+    assert bool(((y.double() - want).abs() <= 1.01 * tol + 2.0 ** -8 * want.abs() + 2.0 ** -134).all())
+    no_device_error()
