@@ -186,8 +186,9 @@ template <int FDT> __device__ __forceinline__ uint32_t scale_pair(int param, uin
 }
 
 // One stored word times its scale, as packed F x2 in element order: dequant_word itself, so that the weight is dequantize's to
-// the bit for every scale.  (8-bit codes in bf16 from one multiply-add, (32768 + b) s - 32896 s, is 0.5 to 2 % faster - 1 row
-// of 14336 x 4096 24.0 us, here 24.1; 16 rows 33.5 and 34.0; 4096 rows 428 and 429 - but 32896 s is no finite f32 from |s| = 2^113 on.)
+// the bit for every scale.  (8-bit codes in bf16 from one multiply-add, (32768 + b) s - 32896 s, is 0.5 to 2 % faster, 6 % where
+// pairs of CTAs wait for the weight - 16 rows of 14336 x 4096 33.5 us, here 34.0; 4096 rows 428 and 429; 8 experts of 160 rows
+// 309 and 328 - but 32896 s is no finite f32 from |s| = 2^113 on.  One step or two, by each run's scales: 34.7 and 319.)
 template <int FDT, int KIND> __device__ __forceinline__ void decode_word(uint32_t w, uint32_t s2, uint32_t *o)
 {
     dequant_word<FDT, KIND>(w, widen_lo<FDT>(s2), s2, o);

@@ -69,8 +69,9 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     m.split = 1;
     while (m.split < 8 && tiles <= resident_clusters(m.split * 2, cfg) && m.kblocks / (m.split * 2) >= 4) m.split *= 2;
     // Pairs of CTAs from 160 rows (of an expert, on average): 8 experts 14336 x 4096 q4 with 128 and 159 rows on the other kernel
-    // 264 and 270 us, 128 and 192 rows on pairs 277 and 293; one 4096 x 4096 with 159 rows 27, on pairs 27.  Pairs store a row's
-    // features from one lane, which rows that start on no 16 bytes would turn into single elements all over memory.
+    // 245 and 279 us, with 160 and 192 on pairs 299 and 308; one 4096 x 4096 with 159 rows 31, with 160 on pairs
+    // 28.  Pairs store a row's features from one lane, which rows that start on no 16 bytes would turn into single elements all
+    // over memory.
     // Pairs do not split the contraction, so few tiles of a long one are left to the other kernel: a step of it takes twice as
     // long (0.7 to 0.85 us, of a pair 0.30 to 0.37), and the exchange of a split sum as long as some 64.  us of the other
     // kernel and of pairs, a call at a time: 1024 x 14336 with 160 rows 39 and 76, 512 rows 77 and 92, 1024 rows 63 and 94,
@@ -134,8 +135,8 @@ static cudaError_t launch_mma(int fdt, int kind, bool backward, const LinearArgs
     return launches[wide][backward][fdt == QK_BF16](kind, xmap, wmap, m, grid, smem, cfg, stream);
 }
 
-// A handful of rows (of an expert, on average): 14336 x 4096 q8 with 8 rows 22 us, with 9 on the tiles of the tensor
-// cores 31; of each of 8 experts, q4, 148 and 202 us, q8 both 195.
+// A handful of rows (of an expert, on average): 14336 x 4096 q8 with 8 rows 27 us, with 9 on the tiles of the tensor
+// cores 34; of each of 8 experts, q4, 105 and 189 us, q8 162 and 207.
 static bool handful(bool backward, const LinearArgs &a) { return !backward && a.k > 0 && a.rows <= SKINNY_ROWS * a.experts; }
 
 // Tiles are numbered by 32-bit integers, and a CTA steps past the last one by less than 2^20.

@@ -8,7 +8,7 @@
 // add their sums in warp order through shared memory.
 // Codes are on their way two chunks ahead, by asynchronous copies into the warp's own ring in shared memory: whole rows of a
 // chunk at a time, and no registers, so that 24 warps fit an SM (with a ring in registers 16 did: 127 us for 206 MB of
-// 4-bit codes of 7 experts, 82 now).
+// 4-bit codes of 7 experts, 85 now).
 #pragma once
 
 #include "linear_tiles.cuh"
